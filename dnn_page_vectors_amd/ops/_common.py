@@ -100,6 +100,14 @@ def stream(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (a launch goes to the current device,
+    whatever device its stream belongs to)."""
+    if t.is_cuda and t.device.index != torch.cuda.current_device():
+        return torch.cuda.device(t.device)
+    return contextlib.nullcontext()
+
+
 def P(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

@@ -134,6 +134,19 @@ SIGS = {
     "pv_cast_pad_bf16": "pp" "lii" "p",
     "pv_sumsq": "p" "l" "p" "p",
     "pv_scale": "p" "lf" "p",
+    # window_attention.hip
+    "pv_wattn_fwd": "ppppp" "pli" "p" "iiiii" "iii" "f" "p",
+    "pv_wattn_bwd": "ppppp" "pppp" "pli" "pp" "iiiii" "iii" "f" "p",
+    # token_embedding.hip
+    "pv_temb_fwd": "pipipi" "lli" "f" "pp" "ppi" "p",
+    "pv_temb_grad_ws": "lli",
+    "pv_temb_grad": "pipip" "lli" "l" "f" "i" "pl" "p",
+    # ckpt8.hip
+    "pv_ckpt8_pack": "pipp" "li" "p",
+    "pv_ckpt8_unpack": "pppi" "li" "p",
+    "pv_ckpt8_gelu_fwd": "ppppp" "li" "p",
+    "pv_ckpt8_gelu_bwd_ws": "li",
+    "pv_ckpt8_gelu_bwd": "pppppp" "i" "p" "li" "p",
     # gemm_mx8.hip
     "pv_mx_probe": "ppppp" "p",
     "pv_gemm_mx8": "p" "l" "p" "l" "p" "l" "iii" "i" "l" "p" "f" "p" "ii" "p",
@@ -147,7 +160,7 @@ SIGS = {
 
 _RESTYPE = {"pv_rsort_temp_bytes": ctypes.c_long, "pv_ib_fwd_dq_parts": ctypes.c_long, "pv_ib_bwd_ws": ctypes.c_long, "pv_ib_fwd_ws": ctypes.c_long,
             "pv_bias_gelu_bwd_ws": ctypes.c_long, "pv_layernorm_bwd_ws": ctypes.c_long,
-            "pv_ibw_ws": ctypes.c_long}
+            "pv_ibw_ws": ctypes.c_long, "pv_temb_grad_ws": ctypes.c_long, "pv_ckpt8_gelu_bwd_ws": ctypes.c_long}
 
 
 def declare(lib) -> None:
