@@ -1,0 +1,492 @@
+// Token-embedding lookup with scaling, and its table gradient summed over the sorted tokens.
+//
+//   out[t] = scale W[id[t]]  (+ pos[l(t)] + typ: the transformer's front end)
+//   dW[v]  = scale sum of g[t] over the tokens t with id[t] = v, v != pad
+//
+// The lookup moves T rows out and reads T rows of a table that the caches mostly hold; the
+// gradient reads T rows and writes V: both are bound by memory.
+//
+// Gradient.  Float atomics would make the sums depend on arrival order and serialise on frequent
+// ids (a word of a Zipf text is several percent of all tokens).  Here every row has one writer:
+//   * few tokens (T <= SMALL_T): one launch.  A workgroup per token; the first token of an id adds
+//     all rows of that id, found by comparing ids; other workgroups zero the rows without a token.
+//   * else the tokens are sorted by id (radix_sort.hip, stable), a wave adds the rows of CHUNK
+//     consecutive sorted tokens, writing the runs that lie inside its chunk, and the runs that
+//     cross a chunk's border are joined from the chunks' fp32 partial rows by a second launch.
+// All sums are fp32, in an order that depends on the sizes and ids alone.
+#include "common.h"
+
+PV_API long pv_rsort_temp_bytes(long n, int end_bit, int key_bytes);
+PV_API int pv_rsort_pairs(void* temp, long temp_bytes, const void* keys_in, void* keys_out, const unsigned* vals_in,
+                          unsigned* vals_out, long n, int end_bit, int key_bytes, void* stream);
+
+namespace pv {
+namespace temb {
+
+constexpr int SMALL_T = 2048;
+constexpr int CHUNK = 32;  // sorted tokens per wave
+constexpr int ZROWS = 64;  // table rows per zeroing workgroup of the small path
+
+struct Groups {
+  int off[4], L[4], n;
+};
+
+struct Ids {
+  const void* p;
+  int is64;
+  __device__ __forceinline__ long at(long t) const {
+    return is64 ? reinterpret_cast<const long*>(p)[t] : (long)reinterpret_cast<const int*>(p)[t];
+  }
+  // the table row whose gradient token t adds to; V (none) for the padding id and ids out of range
+  __device__ __forceinline__ unsigned key(long t, long V, long pad) const {
+    const long i = at(t);
+    return (i < 0 || i >= V || i == pad) ? (unsigned)V : (unsigned)i;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float load1(const T* p);
+template <>
+__device__ __forceinline__ float load1<float>(const float* p) { return *p; }
+template <>
+__device__ __forceinline__ float load1<unsigned short>(const unsigned short* p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(unsigned short* p, float v) { *p = f32_to_bf16(v); }
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+__device__ __forceinline__ void load8(const unsigned short* p, float (&x)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(a[i] << 16), x[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
+  reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+}
+__device__ __forceinline__ void store8(unsigned short* p, const float (&x)[8]) {
+  *reinterpret_cast<u32x4*>(p) =
+      u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+
+// ------------------------------------------------------------------------------------ lookup
+// A workgroup owns `rows` consecutive tokens; a thread takes pieces of C columns of them (C = 8: 16-byte
+// stores; C = 1: row lengths or pointers that are no multiple of 16 bytes).
+template <typename TW, typename TO, int C>
+__global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restrict__ W, TO* __restrict__ out, long T,
+                                                     long V, int E, float scale, int rows,
+                                                     const float* __restrict__ pos, const float* __restrict__ typ,
+                                                     Groups gr) {
+  const long t0 = (long)blockIdx.x * rows;
+  const int n = (int)min((long)rows, T - t0), per = E / C;
+  for (int x = threadIdx.x; x < n * per; x += 256) {
+    const int r = x / per, c = (x - r * per) * C;
+    const long t = t0 + r;
+    const long id = ids.at(t);
+    const bool ok = id >= 0 && id < V;
+    float v[C];
+    if constexpr (C == 8) load8(W + (ok ? id : 0) * E + c, v);
+    else v[0] = load1(W + (ok ? id : 0) * E + c);
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = ok ? v[i] * scale : __uint_as_float(0x7FC00000u);
+    if (pos) {
+      int g = 0;
+      while (g + 1 < gr.n && t >= gr.off[g + 1]) ++g;
+      const float* pp = pos + (size_t)((t - gr.off[g]) % gr.L[g]) * E + c;
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = (v[i] + pp[i]) + typ[c + i];
+    }
+    if constexpr (C == 8) store8(out + t * E + c, v);
+    else store1(out + t * E + c, v[0]);
+  }
+}
+
+// ------------------------------------------------------------------------------------ gradient
+// A lane owns W consecutive columns (4, or 1 where rows are not 4-aligned) of NJ column groups of a
+// slab of 64 W NJ columns.
+template <typename TG, int W, int NJ>
+struct Cols {
+  float a[NJ][W];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) a[j][i] = 0.f;
+  }
+  __device__ __forceinline__ static int col(int j) {
+    return blockIdx.y * (64 * W * NJ) + j * 64 * W + (threadIdx.x & 63) * W;
+  }
+  __device__ __forceinline__ void load(const TG* row, int E) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int c = col(j);
+      if (c >= E) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) a[j][i] = 0.f;
+      } else if constexpr (W == 1) {
+        a[j][0] = load1(row + c);
+      } else if constexpr (sizeof(TG) == 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(row + c);
+#pragma unroll
+        for (int i = 0; i < W; ++i) a[j][i] = v[i];
+      } else {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(row + c);
+        a[j][0] = __uint_as_float(v[0] << 16);
+        a[j][1] = __uint_as_float(v[0] & 0xFFFF0000u);
+        a[j][2] = __uint_as_float(v[1] << 16);
+        a[j][3] = __uint_as_float(v[1] & 0xFFFF0000u);
+      }
+    }
+  }
+  template <typename O>
+  __device__ __forceinline__ void add(const O& x) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) a[j][i] += x.a[j][i];
+  }
+  // dst row = (acc ? dst row : 0) + scale * this
+  __device__ __forceinline__ void store(float* row, int E, float scale, bool acc) const {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int c = col(j);
+      if (c >= E) continue;
+      if constexpr (W == 1) {
+        row[c] = (acc ? row[c] : 0.f) + a[j][0] * scale;
+      } else {
+        f32x4 v = acc ? *reinterpret_cast<const f32x4*>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] += a[j][i] * scale;
+        *reinterpret_cast<f32x4*>(row + c) = v;
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Sum over the four waves of a workgroup in wave order, into wave 0's x
+template <typename X, int W, int NJ>
+__device__ __forceinline__ void join_waves(X& x, float (&sh)[3][NJ][W][64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (wave)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) sh[wave - 1][j][i][lane] = x.a[j][i];
+  __syncthreads();
+  if (wave == 0)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int w = 0; w < 3; ++w) x.a[j][i] += sh[w][j][i][lane];
+}
+
+// Few tokens.  Workgroup b < T: token b, which writes its id's row if it is the id's first token
+// (every wave adds the rows of one quarter of the tokens).  Workgroups behind: zeros for the rows
+// without a token.
+template <typename TG, int W, int NJ>
+__global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __restrict__ g, float* __restrict__ dW,
+                                                         int T, long V, int E, long pad, float scale, int acc) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x < T) {
+    __shared__ float sh[3][NJ][W][64];
+    const int t = blockIdx.x;
+    const unsigned v = ids.key(t, V, pad);
+    if (v == (unsigned)V) return;
+    int before = 0;
+    for (int u = threadIdx.x; u < t; u += 256) before |= ids.key(u, V, pad) == v;
+    if (__syncthreads_or(before)) return;
+    const int q = (T - t + 3) / 4, u0 = t + wave * q, u1 = min(T, u0 + q);
+    Cols<TG, W, NJ> sum, row;
+    sum.zero();
+    for (int u = u0; u < u1; u += 64) {
+      unsigned long long hit = __ballot(u + lane < u1 && ids.key(min(u + lane, T - 1), V, pad) == v);
+      while (hit) {
+        const int k = __builtin_ctzll(hit);
+        hit &= hit - 1;
+        row.load(g + (size_t)(u + k) * E, E);
+        sum.add(row);
+      }
+    }
+    join_waves<Cols<TG, W, NJ>, W, NJ>(sum, sh);
+    if (wave == 0) sum.store(dW + (size_t)v * E, E, scale, acc);
+    return;
+  }
+  __shared__ int has[ZROWS];
+  if (blockIdx.y) return;  // the zeroing workgroups take whole rows
+  const long r0 = (long)(blockIdx.x - T) * ZROWS;
+  if (threadIdx.x < ZROWS) has[threadIdx.x] = 0;
+  __syncthreads();
+  for (int u = threadIdx.x; u < T; u += 256) {
+    const long k = (long)ids.key(u, V, pad) - r0;
+    if (k >= 0 && k < ZROWS) has[k] = 1;
+  }
+  __syncthreads();
+  const int n = (int)min((long)ZROWS, V - r0);
+  for (int r = wave; r < n; r += 4) {
+    if (has[r]) continue;
+    float* row = dW + (r0 + r) * E;
+    if constexpr (W == 4) {
+      for (int c = lane * 4; c < E; c += 256) *reinterpret_cast<f32x4*>(row + c) = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else {
+      for (int c = lane; c < E; c += 64) row[c] = 0.f;
+    }
+  }
+}
+
+// Sort keys of the tokens; the same launch zeroes the gradient (z floats at dW)
+template <typename KT>
+__global__ __launch_bounds__(256) void key_kernel(Ids ids, KT* __restrict__ keys, long T, long V, long pad,
+                                                  float* __restrict__ dW, long z) {
+  const long i0 = (long)blockIdx.x * 256 + threadIdx.x, n = (long)gridDim.x * 256;
+  for (long t = i0; t < T; t += n) keys[t] = (KT)ids.key(t, V, pad);
+  const bool vec = (reinterpret_cast<size_t>(dW) & 15) == 0;
+  const long z4 = vec ? z / 4 : 0;
+  for (long i = i0; i < z4; i += n) reinterpret_cast<f32x4*>(dW)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (long i = z4 * 4 + i0; i < z; i += n) dW[i] = 0.f;
+}
+
+// A wave adds the rows of its chunk of the sorted tokens, run by run.  Partial rows: slot 2 c = the
+// part of a run that began before chunk c, slot 2 c + 1 = the part of a run that begins in chunk c
+// and goes on behind it.
+template <typename TG, typename KT, int W, int NJ>
+__global__ __launch_bounds__(256) void walk_kernel(const KT* __restrict__ keys, const unsigned* __restrict__ slot,
+                                                   const TG* __restrict__ g, float* __restrict__ part,
+                                                   float* __restrict__ dW, long T, long V, int E, float scale,
+                                                   int acc) {
+  const int lane = threadIdx.x & 63;
+  const long c = (long)blockIdx.x * 4 + (threadIdx.x >> 6), b = c * CHUNK, e = min(T, b + CHUNK);
+  if (b >= T) return;
+  const unsigned none = (unsigned)V;
+  unsigned mykey = none, mypos = 0;
+  if (lane < CHUNK && b + lane < e) {
+    mykey = keys[b + lane];
+    mypos = slot[b + lane];
+  }
+  unsigned cur = uniform(mykey);
+  if (cur == none) return;  // padding sorts last
+  const bool from_before = b > 0 && keys[b - 1] == (KT)cur;
+  const unsigned behind = e < T ? (unsigned)keys[e] : none;
+  bool first = true;
+  Cols<TG, W, NJ> sum;
+  sum.zero();
+  auto flush = [&](unsigned key, bool goes_on) {
+    if (first && from_before) sum.store(part + (2 * c) * E, E, 1.f, false);
+    else if (goes_on) sum.store(part + (2 * c + 1) * E, E, 1.f, false);
+    else sum.store(dW + (size_t)key * E, E, scale, acc);
+    first = false;
+    sum.zero();
+  };
+  const int n = (int)(e - b);
+  constexpr int U = NJ >= 4 ? 4 : 8;  // rows in flight
+  for (int k0 = 0; k0 < n; k0 += U) {
+    Cols<TG, W, NJ> row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned p = __builtin_amdgcn_readlane(mypos, min(k0 + u, n - 1));
+      row[u].load(g + (size_t)p * E, E);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u >= n) break;
+      const unsigned k = __builtin_amdgcn_readlane(mykey, k0 + u);
+      if (k != cur) {
+        flush(cur, false);
+        cur = k;
+      }
+      if (cur == none) return;
+      sum.add(row[u]);
+    }
+  }
+  flush(cur, behind == cur);
+}
+
+// A workgroup per chunk: where a run begins in chunk c and goes on behind it, the sum of its partial
+// rows (each wave adds one quarter of them).
+template <typename TG, typename KT, int W, int NJ>
+__global__ __launch_bounds__(256) void join_kernel(const KT* __restrict__ keys, const float* __restrict__ part,
+                                                   float* __restrict__ dW, long T, long V, int E, float scale,
+                                                   int acc) {
+  __shared__ float sh[3][NJ][W][64];
+  const long c = blockIdx.x, b = c * CHUNK, e = b + CHUNK;
+  if (e >= T) return;
+  const KT key = keys[e - 1];
+  if ((unsigned)key == (unsigned)V || keys[e] != key) return;
+  if (keys[b] == key && b > 0 && keys[b - 1] == key) return;  // began before this chunk
+  long lo = e, hi = T;  // first position behind the run
+  while (lo < hi) {
+    const long mid = (lo + hi) >> 1;
+    if (keys[mid] == key) lo = mid + 1;
+    else hi = mid;
+  }
+  const long m = (lo - 1) / CHUNK - c + 1;  // partial rows: slot 2c+1, then 2(c+1), 2(c+2), ..
+  const int wave = threadIdx.x >> 6;
+  const long q = (m + 3) / 4, x0 = wave * q, x1 = min(m, x0 + q);
+  Cols<float, W, NJ> sum, row;
+  sum.zero();
+#pragma unroll 4
+  for (long x = x0; x < x1; ++x) {
+    row.load(part + (x == 0 ? 2 * c + 1 : 2 * (c + x)) * E, E);
+    sum.add(row);
+  }
+  join_waves<Cols<float, W, NJ>, W, NJ>(sum, sh);
+  if (wave == 0) sum.store(dW + (size_t)key * E, E, scale, acc);
+}
+
+__host__ inline size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct Layout {
+  size_t keys, skeys, slot, part, temp, bytes;
+  long temp_bytes, chunks;
+  int kb, bits;
+};
+
+__host__ inline Layout layout(long T, long V, int E) {
+  Layout l{};
+  if (T <= SMALL_T) return l;
+  l.kb = V < 65536 ? 2 : 4;
+  while ((1L << l.bits) <= V) ++l.bits;  // keys 0 .. V
+  l.chunks = (T + CHUNK - 1) / CHUNK;
+  size_t o = 0;
+  l.keys = o;
+  o = up(o + (size_t)T * l.kb);
+  l.skeys = o;
+  o = up(o + (size_t)T * l.kb);
+  l.slot = o;
+  o = up(o + (size_t)T * 4);
+  l.part = o;
+  o = up(o + (size_t)l.chunks * 2 * E * 4);
+  l.temp = o;
+  l.temp_bytes = pv_rsort_temp_bytes(T, l.bits, l.kb);
+  l.bytes = up(o + (size_t)l.temp_bytes);
+  return l;
+}
+
+template <typename TG, typename KT, int W, int NJ>
+int sorted_grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc,
+                char* ws, const Layout& l, hipStream_t st) {
+  KT *keys = (KT*)(ws + l.keys), *sk = (KT*)(ws + l.skeys);
+  unsigned* slot = (unsigned*)(ws + l.slot);
+  float* part = (float*)(ws + l.part);
+  const long z = acc ? 0 : V * E;
+  const long want = (max(T, z / 4) + 255) / 256;
+  hipLaunchKernelGGL((key_kernel<KT>), dim3((unsigned)min(want, 4096L)), dim3(256), 0, st, ids, keys, T, V, pad, dW, z);
+  PV_LAUNCH_CHECK();
+  if (const int rc = pv_rsort_pairs(ws + l.temp, l.temp_bytes, keys, sk, nullptr, slot, T, l.bits, l.kb, st)) return rc;
+  const int slabs = (E + 64 * W * NJ - 1) / (64 * W * NJ);
+  hipLaunchKernelGGL((walk_kernel<TG, KT, W, NJ>), dim3((unsigned)((l.chunks + 3) / 4), slabs), dim3(256), 0, st,
+                     (const KT*)sk, (const unsigned*)slot, g, part, dW, T, V, E, scale, acc);
+  PV_LAUNCH_CHECK();
+  hipLaunchKernelGGL((join_kernel<TG, KT, W, NJ>), dim3((unsigned)l.chunks, slabs), dim3(256), 0, st, (const KT*)sk,
+                     (const float*)part, dW, T, V, E, scale, acc);
+  PV_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename TG, int W, int NJ>
+int grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
+         long ws_bytes, hipStream_t st) {
+  if (T <= SMALL_T) {
+    const int slabs = (E + 64 * W * NJ - 1) / (64 * W * NJ);
+    const long z = acc ? 0 : (V + ZROWS - 1) / ZROWS;
+    if (T + z > 0x7FFFFFFFL) return -4;
+    if (T + z == 0) return 0;
+    hipLaunchKernelGGL((small_grad_kernel<TG, W, NJ>), dim3((unsigned)(T + z), slabs), dim3(256), 0, st, ids, g, dW,
+                       (int)T, V, E, pad, scale, acc);
+    PV_LAUNCH_CHECK();
+    return 0;
+  }
+  const Layout l = layout(T, V, E);
+  if (!ws || (size_t)ws_bytes < l.bytes) return -5;
+  return l.kb == 2 ? sorted_grad<TG, unsigned short, W, NJ>(ids, g, dW, T, V, E, pad, scale, acc, ws, l, st)
+                   : sorted_grad<TG, unsigned, W, NJ>(ids, g, dW, T, V, E, pad, scale, acc, ws, l, st);
+}
+
+template <typename TG, int W>
+int grad_nj(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
+            long ws_bytes, hipStream_t st) {
+  const int groups = (E + 64 * W - 1) / (64 * W);
+  if (groups == 1) return grad<TG, W, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+  if (groups == 2) return grad<TG, W, 2>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+  if (groups == 3) return grad<TG, W, 3>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+  return grad<TG, W, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+}
+
+template <typename TG>
+int grad_w(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
+           long ws_bytes, hipStream_t st) {
+  const bool vec = E % 4 == 0 && ((size_t)g % (4 * sizeof(TG))) == 0 && ((size_t)dW % 16) == 0;
+  return vec ? grad_nj<TG, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st)
+             : grad_nj<TG, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+}
+
+template <typename TW, typename TO>
+int lookup(const Ids& ids, const TW* W, TO* out, long T, long V, int E, float scale, const float* pos,
+           const float* typ, const Groups& gr, hipStream_t st) {
+  const bool vec = E % 8 == 0 && ((size_t)W % 16) == 0 && ((size_t)out % 16) == 0;
+  const int per = vec ? E / 8 : E;
+  const int rows = max(1, min(64, 1024 / per));  // about four pieces per thread
+  const dim3 grid((unsigned)((T + rows - 1) / rows));
+  if (vec)
+    hipLaunchKernelGGL((lookup_kernel<TW, TO, 8>), grid, dim3(256), 0, st, ids, W, out, T, V, E, scale, rows, pos, typ, gr);
+  else
+    hipLaunchKernelGGL((lookup_kernel<TW, TO, 1>), grid, dim3(256), 0, st, ids, W, out, T, V, E, scale, rows, pos, typ, gr);
+  PV_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace temb
+}  // namespace pv
+
+using namespace pv;
+using namespace pv::temb;
+
+namespace {
+inline int temb_sizes(long T, long V, long E) {
+  if (T < 0 || V <= 0 || E <= 0) return -1;
+  if (T > 0x7FFFFFFFL || V >= 0x7FFFFFFFL || E > (1L << 20)) return -2;
+  return 0;
+}
+}  // namespace
+
+// ids (T) int32 / int64; W (V, E) fp32 (w16 = 0) or bf16; out (T, E) bf16 (o16 = 1) or fp32.  pos (Lmax, E) and
+// typ (E) fp32, both or none; groups: ng <= 4 (first token, length) pairs, first tokens ascending from 0.  An
+// id outside [0, V) gives a row of NaN.
+PV_API int pv_temb_fwd(const void* ids, int is64, const void* W, int w16, void* out, int o16, long T, long V, int E,
+                       float scale, const float* pos, const float* typ, const int* goff, const int* glen, int ng,
+                       void* stream) {
+  if (const int rc = temb_sizes(T, V, E)) return rc;
+  if (T == 0) return 0;
+  Groups gr{};
+  if (pos) {
+    if (!typ || ng < 1 || ng > 4) return -3;
+    gr.n = ng;
+    for (int i = 0; i < ng; ++i) gr.off[i] = goff[i], gr.L[i] = glen[i];
+  }
+  const Ids id{ids, is64};
+  hipStream_t st = (hipStream_t)stream;
+  if (w16 && o16) return lookup(id, (const unsigned short*)W, (unsigned short*)out, T, V, E, scale, pos, typ, gr, st);
+  if (w16) return lookup(id, (const unsigned short*)W, (float*)out, T, V, E, scale, pos, typ, gr, st);
+  if (o16) return lookup(id, (const float*)W, (unsigned short*)out, T, V, E, scale, pos, typ, gr, st);
+  return lookup(id, (const float*)W, (float*)out, T, V, E, scale, pos, typ, gr, st);
+}
+
+// workspace bytes of pv_temb_grad
+PV_API long pv_temb_grad_ws(long T, long V, int E) { return temb_sizes(T, V, E) ? 0 : (long)layout(T, V, E).bytes; }
+
+// g (T, E) bf16 (g16 = 1) or fp32; dW (V, E) fp32: every row written (acc = 0) or the rows of the tokens added
+// to (acc = 1).  pad: the id whose row gets no gradient, -1 for none.
+PV_API int pv_temb_grad(const void* ids, int is64, const void* g, int g16, float* dW, long T, long V, int E, long pad,
+                        float scale, int acc, void* ws, long ws_bytes, void* stream) {
+  if (const int rc = temb_sizes(T, V, E)) return rc;
+  const Ids id{ids, is64};
+  hipStream_t st = (hipStream_t)stream;
+  return g16 ? grad_w(id, (const unsigned short*)g, dW, T, V, E, pad, scale, acc, (char*)ws, ws_bytes, st)
+             : grad_w(id, (const float*)g, dW, T, V, E, pad, scale, acc, (char*)ws, ws_bytes, st);
+}

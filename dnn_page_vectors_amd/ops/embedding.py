@@ -27,7 +27,7 @@ import torch
 from . import dense as dops
 from . import grad_sink
 from . import reference as ref
-from ._common import P, check, lib, stream, use_hip
+from ._common import P, check, lib, on_device, stream, use_hip
 from ..parallel.sparse_rows import note_rows
 from .conv_pool import sort_pairs_iota
 
@@ -440,3 +440,104 @@ def trigram_hash(text: torch.Tensor, lens: torch.Tensor, L: int, hash_size: int)
                                     hash_size, stream(text.device)), "pv_trigram_hash")
         return out
     return ref.fnv1a_trigram_ids(text.cpu(), lens.cpu(), L, hash_size).to(text.device)
+
+
+# ---- scaled token lookup, gradient summed over the sorted tokens (csrc/kernels/token_embedding.hip) --------
+
+def lookup_rows(ids: torch.Tensor, W: torch.Tensor, out: torch.Tensor, scale: float, pos=None, typ0=None,
+                groups=()) -> None:
+    """out (T, E) bf16 / fp32 = scale * W[ids] (+ pos[position] + typ0: position of token t of group
+    (N_i, L_i) of the packed ids = its place in its sequence).  One launch."""
+    import ctypes
+
+    offs, off = [], 0
+    for N, L in groups:
+        offs.append(off)
+        off += N * L
+    oa = (ctypes.c_int * len(offs))(*offs) if offs else None
+    la = (ctypes.c_int * len(offs))(*[L for _, L in groups]) if offs else None
+    with on_device(W):
+        check(lib().pv_temb_fwd(P(ids), int(ids.dtype == torch.int64), P(W), int(W.dtype == torch.bfloat16), P(out),
+                                int(out.dtype == torch.bfloat16), out.shape[0], W.shape[0], W.shape[1], float(scale),
+                                P(pos), P(typ0), oa, la, len(offs), stream(W.device)), "pv_temb_fwd")
+
+
+def sorted_row_grad(ids: torch.Tensor, g: torch.Tensor, dst: torch.Tensor, scale: float, padding_idx: Optional[int],
+                    accumulate: bool) -> torch.Tensor:
+    """dst (V, E) fp32: dst[v] (+)= scale * sum of the rows g[t] with ids[t] = v, in an order that the sizes and
+    ids alone decide (no atomics); ``accumulate`` False writes every row, zeros included.  The padding id
+    and ids outside the table add nothing."""
+    T, E = g.shape
+    V = dst.shape[0]
+    with on_device(dst):
+        n = int(lib().pv_temb_grad_ws(T, V, E))
+        ws = torch.empty(n, dtype=torch.uint8, device=dst.device) if n else None
+        check(lib().pv_temb_grad(P(ids), int(ids.dtype == torch.int64), P(g), int(g.dtype == torch.bfloat16), P(dst),
+                                 T, V, E, -1 if padding_idx is None else int(padding_idx), float(scale),
+                                 int(accumulate), P(ws), n, stream(dst.device)), "pv_temb_grad")
+    return dst
+
+
+class _ScaledEmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, W, ids, scale, padding_idx, out_dtype):
+        out = torch.empty(ids.numel(), W.shape[1], dtype=out_dtype, device=W.device)
+        lookup_rows(ids, W.contiguous(), out, scale)
+        ctx.save_for_backward(ids)
+        ctx.W = W  # flat-gradient direct-write target (ops/grad_sink.py)
+        ctx.meta = (scale, padding_idx)
+        return out.view(*ids.shape, W.shape[1])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        W = ctx.W
+        g = g.reshape(-1, W.shape[1]).contiguous()
+        if g.dtype not in (torch.bfloat16, torch.float32):
+            g = g.float()
+        tw = grad_sink.accum_target(W)
+        if tw is not None:
+            sorted_row_grad(ids, g, tw, *ctx.meta, accumulate=True)
+            grad_sink.done(W)
+            return None, None, None, None, None
+        dW = torch.empty(W.shape, dtype=torch.float32, device=W.device)
+        sorted_row_grad(ids, g, dW, *ctx.meta, accumulate=False)
+        return dW if W.dtype == torch.float32 else dW.to(W.dtype), None, None, None, None
+
+
+def scaled_embedding(ids: torch.Tensor, W: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
+                     out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """scale * W[ids]: ids (...) int32 / int64, W (V, E) fp32 or bf16 -> (..., E) in ``out_dtype``
+    (bf16 or fp32; default bf16 on the GPU, W's type elsewhere).
+
+    The gradient of W is summed in fp32 over the tokens sorted by id: one writer per row, the same
+    bits on every run.  The row ``padding_idx`` gets no gradient.  On the GPU an id outside [0, V) gives
+    a row of NaN (which the trainer's non-finite guard sees) and adds to no gradient; the CPU raises."""
+    if W.dim() != 2 or W.dtype not in (torch.float32, torch.bfloat16) and W.is_cuda or not W.is_floating_point():
+        raise TypeError(f"scaled_embedding: W must be a 2-D float32 or bfloat16 table, got {W.dim()}-D {W.dtype}")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"scaled_embedding: ids must be int32 or int64, got {ids.dtype}")
+    if ids.device != W.device:
+        raise ValueError(f"scaled_embedding: ids are on {ids.device}, the table on {W.device}")
+    V = W.shape[0]
+    if padding_idx is not None and not 0 <= int(padding_idx) < V:
+        raise ValueError(f"scaled_embedding: padding_idx {padding_idx} is outside the table's {V} rows")
+    if not scale == scale or scale in (float("inf"), float("-inf")):
+        raise ValueError(f"scaled_embedding: scale must be finite, got {scale}")
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if use_hip(W) else W.dtype
+    note_rows(W, ids)  # row-sparse table gradients (parallel/sparse_rows.py) record the rows
+    if not use_hip(W):
+        rows = torch.nn.functional.embedding(ids.long(), W, padding_idx=padding_idx)
+        return (rows.to(torch.promote_types(W.dtype, torch.float32)) * scale).to(out_dtype)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"scaled_embedding: out_dtype must be bfloat16 or float32 on the GPU, got {out_dtype}")
+    if W.shape[1] == 0 or V == 0 or ids.numel() >= 1 << 31 or V >= (1 << 31) - 1 or W.shape[1] > 1 << 20:
+        raise ValueError(f"scaled_embedding: {ids.numel()} tokens of a {tuple(W.shape)} table are outside the kernels' range")
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and W.requires_grad:
+        return _ScaledEmbeddingFn.apply(W, ids, float(scale), padding_idx, out_dtype)
+    out = torch.empty(*ids.shape, W.shape[1], dtype=out_dtype, device=W.device)
+    lookup_rows(ids, W.detach().contiguous(), out.view(-1, W.shape[1]), scale)
+    return out
