@@ -94,6 +94,15 @@ class Configuration:
     bert_max_len: int = 512
     bert_out_dim: int = 0                 # 0 => CLS vector (768), else projection
     bert_dropout: float = 0.1
+    # long pages: each token attends to bert_window tokens on either side (0 = all tokens) and to the
+    # first bert_sinks tokens of the page, which stay visible ([CLS] is the first)
+    bert_window: int = 0
+    bert_sinks: int = 1
+    # token embeddings times this (0 = as they are; sqrt(bert_hidden) keeps them ahead of the position
+    # embeddings); the table gradient is then summed over the sorted tokens, the padding row untrained
+    bert_embed_scale: float = 0.0
+    # keep the linear layers' inputs and the GELU's input in 8 bits for the backward (ops/ckpt8.py)
+    bert_ckpt8: bool = False
     # chunked long-page encoder (config 5)
     chunk_len: int = 512
     num_chunks: int = 8
@@ -169,6 +178,8 @@ class Configuration:
             raise ValueError("use_fp8 (fp8 chunk GEMMs) runs on the HIP path: it needs dtype='bf16'")
         if self.chunk_encoder not in ("mlp", "cdssm"):
             raise ValueError(f"chunk_encoder must be 'mlp' or 'cdssm', got {self.chunk_encoder!r}")
+        if self.bert_window < 0 or self.bert_sinks < 0:
+            raise ValueError("bert_window (0 = dense attention) and bert_sinks must be >= 0")
         if self.num_workers < 0 or self.prefetch < 1:
             raise ValueError("num_workers must be >= 0 (0 = auto) and prefetch >= 1")
 
@@ -363,6 +374,13 @@ def preset_config(name: str) -> Configuration:
                              query_length=32, document_length=256, batch_size=256,
                              dtype="bf16", loss_mode="cross_gpu", J=0, lr=3e-5,
                              inbatch_gamma=20.0, cos_clip=False)
+    if name in ("bert_longpage",):
+        # the dual encoder on whole ngram-length pages: windowed attention (256 tokens to each side
+        # and [CLS]), 8-bit activation checkpoints; the training recipe is bert_dp8's
+        return Configuration(model="bert", feature_level="word", vocab_hash_size=30522,
+                             query_length=32, document_length=2000, bert_max_len=2000, batch_size=64,
+                             dtype="bf16", loss_mode="cross_gpu", J=0, lr=3e-5, inbatch_gamma=20.0, cos_clip=False,
+                             bert_window=256, bert_sinks=1, bert_embed_scale=27.712812921102035, bert_ckpt8=True)
     if name in ("longpage_fp8", "config5"):
         return Configuration(model="chunked", feature_level="ngram", vocab_hash_size=30000,
                              embedding_dim=512, mlp_dims=(512, 512, 128), chunk_len=512,
@@ -391,4 +409,4 @@ def preset_config(name: str) -> Configuration:
 
 
 PRESETS = ["reference_char", "reference_v1", "tiny_dssm_cpu", "cdssm_ngram_bf16",
-           "mlp_xgpu", "bert_dp8", "longpage_fp8", "longpage_cdssm", "lstm"]
+           "mlp_xgpu", "bert_dp8", "bert_longpage", "longpage_fp8", "longpage_cdssm", "lstm"]

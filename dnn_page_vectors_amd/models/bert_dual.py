@@ -15,6 +15,11 @@ are fp32 in the flat parameter buffer (one bucketed all-reduce stream, ~440 MB/s
 BERT-base, overlapped with the backward by parallel/ddp.py).
 Token ids come from the hashed word featurizer (no WordPiece vocab is available
 offline); id 0 = [PAD], position 0 of every sequence is treated as [CLS].
+
+Long pages (``bert_window`` / ``bert_sinks`` / ``bert_ckpt8`` / ``bert_embed_scale``, preset
+``bert_longpage``): attention over a window and the first tokens (ops/window_attention.py: linear in
+the page length), the layers' saved activations in 8 bits (ops/ckpt8.py), scaled token
+embeddings whose table gradient is summed over the sorted tokens (ops/embedding.py).
 """
 from __future__ import annotations
 
@@ -22,16 +27,19 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops import grad_sink
+from ..ops import ckpt8, grad_sink
 from ..ops import transformer as tops
+from ..ops.embedding import scaled_embedding
+from ..ops.window_attention import packed_window_attention
 from ..parallel.sparse_rows import note_rows
 from .base import TwoTowerModel
 
 
 class BertLayer(nn.Module):
-    def __init__(self, H: int, I: int, heads: int):
+    def __init__(self, H: int, I: int, heads: int, window: int = 0, sinks: int = 1, ckpt: bool = False):
         super().__init__()
         self.heads = heads
+        self.window, self.sinks, self.ckpt8 = window, sinks, ckpt
         self.wqkv = nn.Parameter(torch.empty(3 * H, H))
         self.bqkv = nn.Parameter(torch.zeros(3 * H))
         self.wo = nn.Parameter(torch.empty(H, H))
@@ -50,16 +58,26 @@ class BertLayer(nn.Module):
         N, L, H = x.shape
         p = p_drop if training else 0.0
         r1, r2, bl = tops.ResidualLink(), tops.ResidualLink(), tops.BiasGradLink()
-        qkv = tops.linear(x, self.wqkv, self.bqkv, res=r1, bias_link=bl)  # (N, L, 3H) [slot][head][d]
-        a = tops.fused_attention(qkv, mask, self.heads, bias_link=bl)     # (N, L, H), no permute copies
+        if self.window or self.ckpt8:
+            a = self._attend(x.reshape(N * L, H), [mask], [(N, L)], r1).view(N, L, H)
+        else:
+            qkv = tops.linear(x, self.wqkv, self.bqkv, res=r1, bias_link=bl)  # (N, L, 3H) [slot][head][d]
+            a = tops.fused_attention(qkv, mask, self.heads, bias_link=bl)     # (N, L, H), no permute copies
         o = tops.linear(a, self.wo)
         # output bias + hidden dropout fused into the residual add + LayerNorm (counter-hash
         # masks; the bias gradient is reduced in the LayerNorm backward)
         x = tops.add_layernorm(o, x, self.ln1_g, self.ln1_b, p=p, seed=seed, bias=self.bo, res=r1)
-        f2 = tops.ffn(x, self.w1, self.b1, self.w2, res=r2)  # GELU in the GEMM epilogues
+        f2 = (ckpt8 if self.ckpt8 else tops).ffn(x, self.w1, self.b1, self.w2, res=r2)  # GELU in the GEMM epilogues
         return tops.add_layernorm(f2, x, self.ln2_g, self.ln2_b, p=p, seed=(seed + 0x5BD1E995) & 0xFFFFFFFF,
                                   bias=self.b2, res=r2)
 
+    def _attend(self, x: torch.Tensor, masks, shapes, res):
+        """x (T, H) -> attention output (T, H) with the layer's window and checkpoints."""
+        lin = ckpt8.linear if self.ckpt8 else tops.linear
+        qkv = lin(x, self.wqkv, self.bqkv, res=res)
+        if self.window:
+            return packed_window_attention(qkv, masks, shapes, self.heads, self.window, self.window, self.sinks)
+        return tops.packed_attention(qkv, masks, shapes, self.heads)
 
     def forward_packed(self, x: torch.Tensor, masks, shapes, p_drop: float, training: bool, seed: int = 0):
         """x (T, H): several sequence groups packed token-major (see BertEncoder.forward_multi)."""
@@ -67,11 +85,14 @@ class BertLayer(nn.Module):
         # each x feeds a linear layer and a residual add: their gradients meet in the
         # linear's dX GEMM (tops.ResidualLink) instead of an autograd add
         r1, r2, bl = tops.ResidualLink(), tops.ResidualLink(), tops.BiasGradLink()
-        qkv = tops.linear(x, self.wqkv, self.bqkv, res=r1, bias_link=bl)  # (T, 3H): one GEMM, all groups
-        a = tops.packed_attention(qkv, masks, shapes, self.heads, bias_link=bl)
+        if self.window or self.ckpt8:
+            a = self._attend(x, masks, shapes, r1)
+        else:
+            qkv = tops.linear(x, self.wqkv, self.bqkv, res=r1, bias_link=bl)  # (T, 3H): one GEMM, all groups
+            a = tops.packed_attention(qkv, masks, shapes, self.heads, bias_link=bl)
         o = tops.linear(a, self.wo)
         x = tops.add_layernorm(o, x, self.ln1_g, self.ln1_b, p=p, seed=seed, bias=self.bo, res=r1)
-        f2 = tops.ffn(x, self.w1, self.b1, self.w2, res=r2)  # GELU in the GEMM epilogues
+        f2 = (ckpt8 if self.ckpt8 else tops).ffn(x, self.w1, self.b1, self.w2, res=r2)  # GELU in the GEMM epilogues
         return tops.add_layernorm(f2, x, self.ln2_g, self.ln2_b, p=p, seed=(seed + 0x5BD1E995) & 0xFFFFFFFF,
                                   bias=self.b2, res=r2)
 
@@ -114,19 +135,26 @@ class _RowGather(torch.autograd.Function):
 
 class BertEncoder(nn.Module):
     def __init__(self, vocab_size: int, H: int, I: int, heads: int, layers: int, max_len: int, out_dim: int,
-                 gen: torch.Generator):
+                 gen: torch.Generator, window: int = 0, sinks: int = 1, ckpt: bool = False, embed_scale: float = 0.0):
         super().__init__()
+        self.embed_scale = float(embed_scale)
         self.word = nn.Parameter(torch.empty(vocab_size, H))
         self.pos = nn.Parameter(torch.empty(max_len, H))
         self.typ = nn.Parameter(torch.empty(2, H))
         self.ln_g = nn.Parameter(torch.ones(H))
         self.ln_b = nn.Parameter(torch.zeros(H))
-        self.layers = nn.ModuleList([BertLayer(H, I, heads) for _ in range(layers)])
+        self.layers = nn.ModuleList([BertLayer(H, I, heads, window, sinks, ckpt) for _ in range(layers)])
         self.proj = nn.Parameter(torch.empty(out_dim, H)) if out_dim else None
         with torch.no_grad():
             for n, p in self.named_parameters():
                 if p.dim() == 2:
                     p.normal_(0.0, 0.02, generator=gen)
+
+    def _tokens(self, ids: torch.Tensor) -> torch.Tensor:
+        """fp32 token rows (N, L, H)."""
+        if self.embed_scale:
+            return scaled_embedding(ids, self.word, self.embed_scale, padding_idx=0, out_dtype=torch.float32)
+        return _row_gather(ids, self.word)
 
     def forward(self, ids: torch.Tensor, p_drop: float, training: bool, seed: int = 0) -> torch.Tensor:
         dt = torch.bfloat16 if ids.is_cuda else torch.float32
@@ -134,7 +162,7 @@ class BertEncoder(nn.Module):
         N, L = ids.shape
         mask = (ids != 0)
         mask[:, 0] = True  # [CLS] position always attends
-        x = (_row_gather(ids, self.word) + self.pos[:L].unsqueeze(0) + self.typ[0]).to(dt)
+        x = (self._tokens(ids) + self.pos[:L].unsqueeze(0) + self.typ[0]).to(dt)
         x = tops.add_layernorm(x, None, self.ln_g, self.ln_b)
         if training and p_drop > 0:
             x = F.dropout(x, p_drop, True)
@@ -159,12 +187,12 @@ class BertEncoder(nn.Module):
             masks.append(mask)
             shapes.append((N, L))
         # one fused gather + position / type add + cast over every group (ops/transformer.py)
-        x = tops.bert_embed(self.word, self.pos, self.typ, ids_list)
+        x = tops.bert_embed(self.word, self.pos, self.typ, ids_list, self.embed_scale)
         if x is None:
             for ids in ids_list:
                 ids = ids.long()
                 N, L = ids.shape
-                xs.append((_row_gather(ids, self.word) + self.pos[:L].unsqueeze(0) + self.typ[0]).to(dt)
+                xs.append((self._tokens(ids) + self.pos[:L].unsqueeze(0) + self.typ[0]).to(dt)
                           .reshape(N * L, -1))
             x = torch.cat(xs, 0) if len(xs) > 1 else xs[0]
         x = tops.add_layernorm(x, None, self.ln_g, self.ln_b)
@@ -187,7 +215,8 @@ class BertDualEncoder(TwoTowerModel):
         gen = torch.Generator().manual_seed(int(cfg.seed))
         self.vocab_size = vocab_size
         mk = lambda: BertEncoder(vocab_size, cfg.bert_hidden, cfg.bert_intermediate, cfg.bert_heads,
-                                 cfg.bert_layers, cfg.bert_max_len, cfg.bert_out_dim, gen)
+                                 cfg.bert_layers, cfg.bert_max_len, cfg.bert_out_dim, gen, cfg.bert_window,
+                                 cfg.bert_sinks, cfg.bert_ckpt8, cfg.bert_embed_scale)
         self.query_tower = mk()
         # siamese by default: the page tower IS the query tower (one set of weights)
         self.doc_towers = nn.ModuleList([self.query_tower] if cfg.share_doc_tower else [mk()])
@@ -220,4 +249,5 @@ class BertDualEncoder(TwoTowerModel):
 
 def bert_flops_per_token(cfg, L: int) -> float:
     H, I, Lyr = cfg.bert_hidden, cfg.bert_intermediate, cfg.bert_layers
-    return Lyr * (2 * (4 * H * H + 2 * H * I) + 4 * L * H)
+    seen = min(L, 2 * cfg.bert_window + 1 + cfg.bert_sinks) if cfg.bert_window else L
+    return Lyr * (2 * (4 * H * H + 2 * H * I) + 4 * seen * H)

@@ -97,7 +97,9 @@ def lib():
 
 
 def stream(device: Optional[torch.device] = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle: building a torch.cuda.Stream object for it costs 2-9 us per launch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None or device.index is None
+                                              else device.index)
 
 
 def on_device(t: torch.Tensor):

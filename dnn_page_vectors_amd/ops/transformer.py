@@ -410,25 +410,83 @@ class _BertEmbedFn(torch.autograd.Function):
             else:
                 dword = dst
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dpos = torch.zeros(pos.shape, dtype=torch.float32, device=g.device)
-            off = 0
-            for N, L in ctx.groups:
-                dpos[:L] += torch.sum(g[off:off + N * L].view(N, L, H), dim=0, dtype=torch.float32)
-                off += N * L
-            if ctx.needs_input_grad[2]:
-                dtyp = torch.zeros(typ.shape, dtype=torch.float32, device=g.device)
-                dtyp[0] = dpos.sum(0)
-            if not ctx.needs_input_grad[1]:
-                dpos = None
+            dpos, dtyp = _position_grads(g, ctx.groups, pos, typ, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return dword, dpos, dtyp, None, None
 
 
-def bert_embed(word: torch.Tensor, pos: torch.Tensor, typ: torch.Tensor, ids_list) -> Optional[torch.Tensor]:
+def _position_grads(g, groups, pos, typ, want_pos: bool, want_typ: bool):
+    """Position rows as per-group sums over the sequences of g (T, H), the type row as their total."""
+    H = g.shape[1]
+    dpos = torch.zeros(pos.shape, dtype=torch.float32, device=g.device)
+    dtyp = None
+    off = 0
+    for N, L in groups:
+        dpos[:L] += torch.sum(g[off:off + N * L].view(N, L, H), dim=0, dtype=torch.float32)
+        off += N * L
+    if want_typ:
+        dtyp = torch.zeros(typ.shape, dtype=torch.float32, device=g.device)
+        dtyp[0] = dpos.sum(0)
+    return (dpos if want_pos else None), dtyp
+
+
+class _ScaledBertEmbedFn(torch.autograd.Function):
+    """_BertEmbedFn with bf16(scale * word[id] + pos[l] + typ[0]) and the word-table gradient summed over the
+    sorted tokens (csrc/kernels/token_embedding.hip): no atomics, so the deterministic mode takes it too.
+    Id 0 (padding) gets no gradient."""
+
+    @staticmethod
+    def forward(ctx, word, pos, typ, ids_flat, groups, scale):
+        from .embedding import lookup_rows
+
+        out = torch.empty(ids_flat.numel(), word.shape[1], dtype=torch.bfloat16, device=word.device)
+        lookup_rows(ids_flat, word, out, scale, pos, typ[0], groups)
+        ctx.save_for_backward(ids_flat)
+        ctx.groups, ctx.scale = groups, scale
+        ctx.params = (word, pos, typ)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        from .embedding import sorted_row_grad
+
+        (ids_flat,) = ctx.saved_tensors
+        word, pos, typ = ctx.params
+        g = g.to(torch.bfloat16).contiguous()
+        dword = dpos = dtyp = None
+        if ctx.needs_input_grad[0]:
+            tw = grad_sink.accum_target(word)
+            dst = tw if tw is not None else torch.empty(word.shape, dtype=torch.float32, device=g.device)
+            sorted_row_grad(ids_flat, g, dst, ctx.scale, 0, accumulate=tw is not None)
+            if tw is not None:
+                grad_sink.done(word)
+            else:
+                dword = dst
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dpos, dtyp = _position_grads(g, ctx.groups, pos, typ, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return dword, dpos, dtyp, None, None, None
+
+
+def bert_embed(word: torch.Tensor, pos: torch.Tensor, typ: torch.Tensor, ids_list,
+               scale: float = 0.0) -> Optional[torch.Tensor]:
     """Packed (T, H) bf16 embeddings of several id batches, or None off the HIP path and in the
     deterministic mode (the word-table gradient here is float atomics; the per-group path's
-    index_add_ is deterministic there)."""
+    index_add_ is deterministic there).  ``scale`` != 0: the token rows times it, their gradient summed
+    over the sorted tokens (_ScaledBertEmbedFn; deterministic)."""
     from . import determinism
 
+    if scale:
+        if not (use_hip(word) and word.dtype == torch.float32 and len(ids_list) <= 4):
+            return None
+        from ..parallel.sparse_rows import note_rows
+
+        flat = torch.cat([i.reshape(-1) for i in ids_list]) if len(ids_list) > 1 else ids_list[0].reshape(-1).contiguous()
+        if flat.dtype not in (torch.int32, torch.int64):
+            flat = flat.to(torch.int32)
+        note_rows(word, flat)
+        if max(i.shape[1] for i in ids_list) > pos.shape[0]:
+            raise ValueError(f"sequences of {max(i.shape[1] for i in ids_list)} tokens: the position table has {pos.shape[0]} rows")
+        return _ScaledBertEmbedFn.apply(word, pos, typ, flat, [tuple(i.shape) for i in ids_list], float(scale))
     if not (use_hip(word) and word.shape[1] % 8 == 0 and len(ids_list) <= 4 and BERT_EMBED) \
             or determinism.enabled():
         return None
