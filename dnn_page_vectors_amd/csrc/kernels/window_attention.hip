@@ -30,6 +30,10 @@ constexpr int TK = 64;   // rows per staged tile
 constexpr int NTH = 256;
 constexpr int RB = 128;  // rows a workgroup owns: 4 waves x 32
 constexpr float LOG2E = 1.4426950408889634f;
+// The running maximum is raised only when a score passes it by more than this (log2 units): until then
+// probabilities may be as large as 2^8, which costs fp32 sums and bf16 roundings nothing, and the
+// accumulators are not rescaled (32 of ~110 vector instructions per block at d = 64).
+constexpr float SLACK = 8.f;
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
@@ -45,8 +49,8 @@ struct Args {
   const void* mask;  // (N, L), mask_bytes 1 or 4, rows mask_n elements apart; null: all keys
   long mask_n;
   int mask_bytes;
-  float* lse;  // (N, H, L), log2 domain, includes the scale; null: not kept
-  float* dd;   // (N, H, L)  D
+  float* lse;  // (N, H, L)  minus the log-sum-exp of a row's scores (log2 units, scale included); null: not kept
+  float* dd;   // (N, H, L)  minus D
   int L, H, G;  // G = query heads per key/value head
   int left, right, sinks;
   float scale;
@@ -55,67 +59,120 @@ struct Args {
 
 #define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16((a), (b), (c), 0, 0, 0)
 
-__device__ __forceinline__ int mask_at(const Args& a, int n, int r) {
-  const long i = (long)n * a.mask_n + r;
-  return a.mask_bytes == 1 ? (int)reinterpret_cast<const unsigned char*>(a.mask)[i]
-                           : reinterpret_cast<const int*>(a.mask)[i];
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// ---- tiles in LDS ---------------------------------------------------------------------------
+// [64 rows][D] bf16, rows of D / 8 16-byte chunks; chunk c of row r is stored at place c ^ swz(r), so that
+// both the row reads (8 rows, one chunk each) and the transposed reads (4 rows, 4 chunks each)
+// touch every bank once.
+template <int D>
+__device__ __forceinline__ constexpr int swz(int r) {
+  return D == 32 ? ((r >> 2) & 1) << 1 : D == 64 ? (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1)
+                                                 : ((r & 3) << 2) | (((r >> 2) & 1) << 1);
 }
 
-// Registers of a tile on its way to LDS: D / 32 16-byte pieces per thread.  Rows behind the
-// sequence and masked rows are stored as zeros, so whatever they hold (infinities and NaN
-// too) never meets a zero probability in a product.
+// Tile rows go from memory straight to LDS (global_load_lds_dwordx4: 64 lanes x 16 bytes land in 1 KB in
+// lane order), D / 32 pieces per wave; the swizzle is applied to the source column.
 template <int D>
-struct Stage {
-  u32x4 v[D / 32];
+struct Loader {
+  static constexpr int P = D / 32, RP = 512 / D;  // pieces per wave, rows per piece
+  unsigned off[P];                                 // this lane's source offset within a tile (bytes)
+  __device__ __forceinline__ void init(long ls) {
+    const int lane = threadIdx.x & 63, w = wave_id();
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      const int r = (w * P + u) * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
+      off[u] = (unsigned)(r * (int)ls + c * 8) * 2;
+    }
+  }
+  __device__ __forceinline__ void issue(const unsigned short* base, long ls, int r0, int L, unsigned short* t) const {
+    const int w = wave_id();
+    const unsigned short* b = base + (long)r0 * ls;
+    if (r0 + TK <= L) {
+#pragma unroll
+      for (int u = 0; u < P; ++u) glds(b, off[u], t + (w * P + u) * 512);
+    } else {  // rows behind the sequence: its last row again (their probabilities are zero)
+      const int lane = threadIdx.x & 63;
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        const int r = (w * P + u) * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
+        glds(b, (unsigned)(min(r, L - 1 - r0) * (int)ls + c * 8) * 2, t + (w * P + u) * 512);
+      }
+    }
+  }
+  // In asm: for the builtin the compiler waits for every load under way before it reads any LDS of the same array,
+  // which would make the prefetch of the next tile a wait for it.  No register is written; landed()
+  // and a barrier stand between these loads and the reads of their tile.
+  static __device__ __forceinline__ void glds(const unsigned short* base, unsigned off, unsigned short* lds) {
+    const unsigned to = __builtin_amdgcn_readfirstlane(
+        (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) unsigned short*)lds));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to)
+                 : "memory", "m0");
+  }
 };
 
+// 64 floats x[r0 ..] of a row of L into LDS, by one wave
+__device__ __forceinline__ void floats_to_lds(const float* x, int r0, int L, float* lds) {
+  const unsigned to = __builtin_amdgcn_readfirstlane(
+      (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) float*)lds));
+  const unsigned off = (unsigned)min((int)(threadIdx.x & 63), L - 1 - r0) * 4u;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(x + r0), "s"(to)
+               : "memory", "m0");
+}
+
+// every load of this wave has arrived (in asm: the compiler does not know of the tile loads)
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// the same for the compiler's own loads, which it would otherwise wait for inside the loop
+__device__ __forceinline__ void operands_here() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), the other counters unlimited
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Masked rows become zeros, so whatever they hold (infinities and NaN too) never meets a zero
+// probability in a product.  Uniform over the workgroup; ends with a barrier.
 template <int D>
-__device__ __forceinline__ void tile_load(const unsigned short* base, long ls, int r0, int L, Stage<D>& s) {
+__device__ __forceinline__ void clear_rows(unsigned short* k, unsigned short* v, unsigned long long keep) {
 #pragma unroll
   for (int u = 0; u < D / 32; ++u) {
-    const int c = threadIdx.x + NTH * u;
-    const int r = c / (D / 8), e = (c % (D / 8)) * 8;
-    s.v[u] = *reinterpret_cast<const u32x4*>(base + (long)min(r0 + r, L - 1) * ls + e);
+    const int c = threadIdx.x + NTH * u, r = c / (D / 8);
+    if (!((keep >> r) & 1ull)) {
+      *reinterpret_cast<u32x4*>(k + c * 8) = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(v + c * 8) = u32x4{0, 0, 0, 0};
+    }
   }
+  __syncthreads();
 }
 
+// This lane's addresses within a tile.  A operand of a product: rows (lane & 31), columns 16 s + 8 (lane / 32).
+// Transposed A operand: row = tile column (lane & 31) of a 32-column group; its 8 k-slots are the tile rows
+// that registers 8 s .. 8 s + 7 of a 32 x 32 accumulator hold in this half-wave: 16 s + 4 h + {0..3}, +8.
 template <int D>
-__device__ __forceinline__ void tile_store(unsigned short* t, const Stage<D>& s, unsigned long long keep) {
+struct Frags {
+  unsigned row[D / 16], tr[D / 32];  // bytes
+  __device__ __forceinline__ void init() {
+    const int lane = threadIdx.x & 63, h = lane >> 5, g = lane >> 4;
 #pragma unroll
-  for (int u = 0; u < D / 32; ++u) {
-    const int c = threadIdx.x + NTH * u;
-    const int r = c / (D / 8), e = (c % (D / 8)) * 8;
-    const bool ok = (keep >> r) & 1ull;
-    *reinterpret_cast<u32x4*>(t + r * (D + 8) + e) = ok ? s.v[u] : u32x4{0, 0, 0, 0};
+    for (int s = 0; s < D / 16; ++s) {
+      const int r = lane & 31;
+      row[s] = (unsigned)(r * D * 2 + ((2 * s + h) ^ swz<D>(r)) * 16);
+    }
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      const int r = 4 * (g >> 1) + ((lane & 15) >> 2), c = 32 * e + 16 * (g & 1) + 4 * (lane & 3);
+      tr[e] = (unsigned)(r * D * 2 + ((c >> 3) ^ swz<D>(r)) * 16 + (c & 7) * 2);
+    }
   }
-}
-
-// bits of the tile's rows that exist and are not masked (every wave computes the same word)
-__device__ __forceinline__ unsigned long long tile_keep(const Args& a, int n, int r0) {
-  const int r = r0 + (threadIdx.x & 63);
-  bool ok = r < a.L;
-  if (ok && a.mask) ok = mask_at(a, n, r) != 0;
-  return __ballot(ok);
-}
-
-// A operand: rows r0 .. r0+31 of a tile, columns 16 s + 8 (lane / 32) ..
-template <int D>
-__device__ __forceinline__ bf16x8 row_frag(const unsigned short* t, int r0, int s) {
-  const int lane = threadIdx.x & 63;
-  return *reinterpret_cast<const bf16x8*>(t + (r0 + (lane & 31)) * (D + 8) + s * 16 + (lane >> 5) * 8);
-}
-
-// A operand, transposed: row = tile column c0 + (lane & 31); its 8 k-slots are the tile rows that a
-// 32 x 32 accumulator's registers 8 s .. 8 s + 7 hold in this half-wave: r0 + 16 s + 4 h + {0..3}, +8
-template <int D>
-__device__ __forceinline__ bf16x8 tr_frag(const unsigned short* t, int r0, int s, int c0) {
-  const int lane = threadIdx.x & 63, g = lane >> 4;
-  const unsigned short* p =
-      t + (r0 + 16 * s + 4 * (g >> 1) + ((lane & 15) >> 2)) * (D + 8) + c0 + 16 * (g & 1) + 4 * (lane & 3);
-  const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
-  const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 8 * (D + 8)));
-  return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-}
+  // rows r0 .. r0 + 31 (r0 a multiple of 32; swz repeats every 8 rows)
+  __device__ __forceinline__ bf16x8 rows(const unsigned short* t, int r0, int s) const {
+    return *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(t) + row[s] + r0 * D * 2);
+  }
+  __device__ __forceinline__ bf16x8 trans(const unsigned short* t, int r0, int s, int e) const {
+    const char* p = reinterpret_cast<const char*>(t) + tr[e] + (r0 + 16 * s) * D * 2;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 8 * D * 2));
+    return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+};
 
 // B operand: this lane's row of a global matrix, columns 16 s + 8 (lane / 32) ..; zeros if !ok
 template <int D>
@@ -133,11 +190,17 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& x, int s) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-__device__ __forceinline__ f32x16 zero16() {
+__device__ __forceinline__ f32x16 splat16(float v) {
   f32x16 z;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  for (int r = 0; r < 16; ++r) z[r] = v;
   return z;
+}
+
+// the same row's value in the other half-wave
+__device__ __forceinline__ float other_half(float v, bool hi) {
+  const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __uint_as_float(hi ? r[0] : r[1]);
 }
 
 // accumulator register r of half-wave h holds row (r & 3) + 8 (r >> 2) + 4 h
@@ -152,13 +215,21 @@ __device__ __forceinline__ unsigned bits_between(int lo, int hi) {
 
 enum { EMPTY = 0, PARTIAL = 1, FULL = 2 };
 
-// 32 queries i0 .. i0+31 against 32 keys j0 .. j0+31, kw = the keys' keep bits; uniform arguments
-__device__ __forceinline__ int block_kind(const Args& a, int i0, int j0, unsigned kw) {
-  if (kw == 0u || j0 > i0 + 31 + a.right) return EMPTY;
-  if (j0 + 31 < i0 - a.left && j0 >= a.sinks) return EMPTY;
-  const bool low = j0 >= i0 + 31 - a.left || j0 + 31 < a.sinks;
-  return (kw == 0xFFFFFFFFu && low && j0 + 31 <= i0 + a.right) ? FULL : PARTIAL;
-}
+// What the 32 queries w0 .. of a wave see of 32 keys j0 .. j0+31 with keep bits kw: scalars, a few compares per block
+struct Sees {
+  int none_lo, none_hi, full_lo, full_hi, sinks;
+  __device__ __forceinline__ Sees(const Args& a, int w0) {
+    none_lo = w0 - a.left - 31;
+    none_hi = w0 < a.L ? w0 + 31 + a.right : -1;
+    full_lo = w0 + 31 - a.left;
+    full_hi = w0 + a.right - 31;
+    sinks = a.sinks;
+  }
+  __device__ __forceinline__ int kind(int j0, unsigned kw) const {
+    if (kw == 0u || j0 > none_hi || (j0 < none_lo && j0 >= sinks)) return EMPTY;
+    return (kw == 0xFFFFFFFFu && j0 <= full_hi && (j0 >= full_lo || j0 + 32 <= sinks)) ? FULL : PARTIAL;
+  }
+};
 
 // the keys of j0 .. j0+31 that query i sees, as bits
 __device__ __forceinline__ unsigned seen_keys(const Args& a, int i, int j0, unsigned kw) {
@@ -166,108 +237,162 @@ __device__ __forceinline__ unsigned seen_keys(const Args& a, int i, int j0, unsi
                (bits_between(0, a.sinks - 1 - j0) & bits_between(0, i + a.right - j0)));
 }
 
-// key tiles of the queries i0 .. i1: `sink` tiles from 0, then lo .. hi
-struct Walk {
-  int sink, lo, n;
-  __device__ __forceinline__ int tile(int it) const { return it < sink ? it : lo + it - sink; }
-};
-__device__ __forceinline__ Walk key_walk(const Args& a, int i0, int i1) {
-  Walk w;
-  w.lo = max(0, i0 - a.left) / TK;
-  const int hi = min(a.L - 1, i1 + a.right) / TK;
-  w.sink = min((a.sinks + TK - 1) / TK, w.lo);
-  w.n = w.sink + hi - w.lo + 1;
-  return w;
+// Walks the key tiles that queries b0 .. b0 + RB - 1 see (the tiles of the sinks, then the window's):
+// `each(tile K, tile V, first key, keep bits)`.  While a tile is worked on, the next one is on its way to the
+// other buffer.  The mask is read ahead for 128 tiles at once, as one word per tile in LDS: tiles without
+// a key that counts cost nothing (a page's padding is such a run of tiles).
+template <int D, typename F>
+__device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0, unsigned short (&kt)[2][TK * D],
+                                          unsigned short (&vt)[2][TK * D], unsigned long long (&words)[128], F each) {
+  const int lane = threadIdx.x & 63;
+  const unsigned short* K = a.k.p + n * a.k.n + kvh * a.k.h;
+  const unsigned short* V = a.v.p + n * a.v.n + kvh * a.v.h;
+  Loader<D> lk, lv;
+  lk.init(a.k.l);
+  lv.init(a.v.l);
+  const int lo = max(0, b0 - a.left) / TK, hi = min(a.L - 1, min(b0 + RB, a.L) - 1 + a.right) / TK;
+  const int sink = min((a.sinks + TK - 1) / TK, lo), jump = lo - sink, tiles = sink + hi - lo + 1;
+  unsigned long long some0 = 0ull, some1 = 0ull;  // tiles of this chunk of 128 that are still to come
+  int chunk = 0;                                  // first tile behind the chunk
+  const unsigned long long tail = a.L % TK ? (1ull << (a.L % TK)) - 1ull : ~0ull;
+  const int last = (a.L - 1) / TK;
+  auto refill = [&]() {
+    const int m = min(tiles - chunk, 128);
+    if (a.mask) {
+      __syncthreads();  // the last chunk's words have been read
+      for (int t0 = 0; t0 < m; t0 += 16) {
+        int mk[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int t = chunk + min(t0 + 4 * u + wave_id(), m - 1), r = (t < sink ? t : t + jump) * TK + lane;
+          const long at = (long)n * a.mask_n + min(r, a.L - 1);
+          mk[u] = a.mask_bytes == 1 ? (int)reinterpret_cast<const unsigned char*>(a.mask)[at]
+                                    : reinterpret_cast<const int*>(a.mask)[at];
+          if (r >= a.L) mk[u] = 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const unsigned long long w = __ballot(mk[u] != 0);
+          const int t = t0 + 4 * u + wave_id();
+          if (t < m && lane == 0) words[t] = w;
+        }
+      }
+      __syncthreads();
+      some0 = __ballot(lane < m && words[lane] != 0ull);
+      some1 = __ballot(lane + 64 < m && words[lane + 64] != 0ull);
+    } else {
+      some0 = m >= 64 ? ~0ull : (1ull << m) - 1ull;
+      some1 = m >= 128 ? ~0ull : m > 64 ? (1ull << (m - 64)) - 1ull : 0ull;
+    }
+    chunk += m;
+  };
+  // the next tile of the walk with a key that counts, or -1; its keep bits
+  auto next = [&](unsigned long long& keep) -> int {
+    while ((some0 | some1) == 0ull) {
+      if (chunk >= tiles) return -1;
+      refill();
+    }
+    int t = some0 ? __builtin_ctzll(some0) : 64 + __builtin_ctzll(some1);
+    if (some0) some0 &= some0 - 1;
+    else some1 &= some1 - 1;
+    const int base = chunk - min(chunk, ((chunk - 1) & 127) + 1);
+    const int g = base + t, tile = g < sink ? g : g + jump;
+    if (a.mask) {
+      const unsigned long long w = words[t];
+      keep = ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(w >> 32)) << 32) |
+             (unsigned)__builtin_amdgcn_readfirstlane((unsigned)w);
+    } else {
+      keep = tile == last ? tail : ~0ull;
+    }
+    return tile;
+  };
+  unsigned long long keep = 0ull, keep1;
+  int t0 = -1, t1 = next(keep1), buf = 1;
+  operands_here();
+  while (t0 >= 0 || t1 >= 0) {  // t0: the tile worked on; t1: the tile being read
+    if (t1 >= 0) {
+      lk.issue(K, a.k.l, t1 * TK, a.L, kt[buf ^ 1]);
+      lv.issue(V, a.v.l, t1 * TK, a.L, vt[buf ^ 1]);
+    }
+    if (t0 >= 0) each(kt[buf], vt[buf], t0 * TK, keep);
+    t0 = t1;
+    keep = keep1;
+    if (t1 >= 0) {
+      landed();
+      __syncthreads();
+      buf ^= 1;
+      if (a.mask && keep != ~0ull) clear_rows<D>(kt[buf], vt[buf], keep);
+      t1 = next(keep1);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------ forward
 // Workgroup = 128 queries of one head; a wave owns 32 of them (lane & 31), both half-waves hold the
 // same queries and split the keys of each block.
 template <int D>
-__global__ __launch_bounds__(NTH, 2) void fwd_kernel(Args a) {
-  __shared__ __attribute__((aligned(16))) unsigned short kt[2][TK * (D + 8)];
-  __shared__ __attribute__((aligned(16))) unsigned short vt[2][TK * (D + 8)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+__global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short kt[2][TK * D];
+  __shared__ __attribute__((aligned(1024))) unsigned short vt[2][TK * D];
+  __shared__ unsigned long long words[128];
+  const int lane = threadIdx.x & 63, h = lane >> 5;
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
   const int tile = bid % a.tiles, nh = bid / a.tiles;
-  const int hd = nh % a.H, n = nh / a.H, kvh = hd / a.G;
-  const int b0 = tile * RB, w0 = b0 + wave * 32, i = w0 + (lane & 31);
-  const unsigned short* K = a.k.p + n * a.k.n + kvh * a.k.h;
-  const unsigned short* V = a.v.p + n * a.v.n + kvh * a.v.h;
-  const float sl = a.scale * LOG2E;
+  const int hd = nh % a.H, n = nh / a.H;
+  const int b0 = tile * RB, w0 = b0 + wave_id() * 32, i = w0 + (lane & 31);
+  const float sl = a.scale * LOG2E, slack = fminf(SLACK / sl, 1e30f);
   bf16x8 qf[D / 16];
   glob_frag<D>(a.q.p + n * a.q.n + (long)min(i, a.L - 1) * a.q.l + hd * a.q.h, i < a.L, qf);
   f32x16 o[D / 32];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) o[c] = zero16();
-  float m = -INFINITY, l = 0.f;
-  const Walk wk = key_walk(a, b0, min(b0 + RB, a.L) - 1);
-  Stage<D> sk, sv;
-  int t0 = wk.tile(0) * TK;
-  tile_load<D>(K, a.k.l, t0, a.L, sk);
-  tile_load<D>(V, a.v.l, t0, a.L, sv);
-  unsigned long long keep = tile_keep(a, n, t0);
-  tile_store<D>(kt[0], sk, keep);
-  tile_store<D>(vt[0], sv, keep);
-  __syncthreads();
-  int buf = 0;
-  for (int it = 0; it < wk.n; ++it, buf ^= 1) {
-    const int j0 = t0;
-    const unsigned long long kw = keep;
-    if (it + 1 < wk.n) {
-      t0 = wk.tile(it + 1) * TK;
-      tile_load<D>(K, a.k.l, t0, a.L, sk);
-      tile_load<D>(V, a.v.l, t0, a.L, sv);
-      keep = tile_keep(a, n, t0);
-    }
+  for (int c = 0; c < D / 32; ++c) o[c] = splat16(0.f);
+  float m = -INFINITY, ms = 0.f, l = 0.f;  // m: raw score, lags behind the maximum by at most SLACK; ms = -m sl
+  Frags<D> fr;
+  fr.init();
+  const Sees sees(a, w0);
+  walk_keys<D>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int jb = j0 + 32 * c;
-      const unsigned kwc = (unsigned)(kw >> (32 * c));
-      const int kind = w0 < a.L ? block_kind(a, w0, jb, kwc) : EMPTY;
+      const unsigned kw = (unsigned)(keep >> (32 * c));
+      const int kind = sees.kind(j0 + 32 * c, kw);
       if (kind == EMPTY) continue;
-      f32x16 s = zero16();
+      f32x16 s = splat16(0.f);
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) s = MFMA32(row_frag<D>(kt[buf], 32 * c, t), qf[t], s);
+      for (int t = 0; t < D / 16; ++t) s = MFMA32(fr.rows(k, 32 * c, t), qf[t], s);
       if (kind == PARTIAL) {
-        const unsigned see = seen_keys(a, i, jb, kwc) >> (4 * h);
+        const unsigned see = seen_keys(a, i, j0 + 32 * c, kw) >> (4 * h);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = (see >> reg_bit(r)) & 1u ? s[r] : -INFINITY;
       }
       float bm = s[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float mn = fmaxf(m, bm);
-      const float ms = mn == -INFINITY ? 0.f : mn * sl;
-      if (__ballot(mn > m) != 0ull) {
-        const float corr = __builtin_amdgcn_exp2f(fmaf(m, sl, -ms));  // 0 at the first visible key
+      bm = fmaxf(bm, other_half(bm, h));
+      if (__ballot(bm > m + slack) != 0ull) {
+        const float mn = fmaxf(m, bm);
+        const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * sl);  // 0 at the first visible key
         l *= corr;
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) o[e] *= corr;
         m = mn;
+        ms = m == -INFINITY ? 0.f : -m * sl;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl, -ms));
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl, ms));
         l += s[r];
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const bf16x8 pb = pack8(s, t);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) o[e] = MFMA32(tr_frag<D>(vt[buf], 32 * c, t, 32 * e), pb, o[e]);
+        for (int e = 0; e < D / 32; ++e) o[e] = MFMA32(fr.trans(v, 32 * c, t, e), pb, o[e]);
       }
     }
-    if (it + 1 < wk.n) {
-      tile_store<D>(kt[buf ^ 1], sk, keep);
-      tile_store<D>(vt[buf ^ 1], sv, keep);
-    }
-    __syncthreads();
-  }
-  l += __shfl_xor(l, 32, 64);
+  });
+  l += other_half(l, h);
   if (i >= a.L) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   unsigned short* orow = a.o.p + n * a.o.n + (long)i * a.o.l + hd * a.o.h;
 #pragma unroll
   for (int e = 0; e < D / 32; ++e)
@@ -277,23 +402,22 @@ __global__ __launch_bounds__(NTH, 2) void fwd_kernel(Args a) {
           uint2{pack_bf16x2(o[e][4 * t] * inv, o[e][4 * t + 1] * inv),
                 pack_bf16x2(o[e][4 * t + 2] * inv, o[e][4 * t + 3] * inv)};
   if (a.lse && h == 0)
-    a.lse[((long)n * a.H + hd) * a.L + i] = l == 0.f ? INFINITY : fmaf(m, sl, __log2f(l));
+    a.lse[((long)n * a.H + hd) * a.L + i] = l == 0.f ? -INFINITY : -fmaf(m, sl, __log2f(l));
 }
 
 // ------------------------------------------------------------------------------------ backward: dq, D
 // Same walk as the forward: dS^T in registers, dq^T += K^T dS^T.  D is the lane's own row sum of
-// do * o and goes to memory for the other kernel.
+// do * o and goes to memory for the other kernel; -D is the start value of the dP accumulators.
 template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_dq_kernel(Args a) {
-  __shared__ __attribute__((aligned(16))) unsigned short kt[2][TK * (D + 8)];
-  __shared__ __attribute__((aligned(16))) unsigned short vt[2][TK * (D + 8)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short kt[2][TK * D];
+  __shared__ __attribute__((aligned(1024))) unsigned short vt[2][TK * D];
+  __shared__ unsigned long long words[128];
+  const int lane = threadIdx.x & 63, h = lane >> 5;
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
   const int tile = bid % a.tiles, nh = bid / a.tiles;
-  const int hd = nh % a.H, n = nh / a.H, kvh = hd / a.G;
-  const int b0 = tile * RB, w0 = b0 + wave * 32, i = w0 + (lane & 31), ic = min(i, a.L - 1);
-  const unsigned short* K = a.k.p + n * a.k.n + kvh * a.k.h;
-  const unsigned short* V = a.v.p + n * a.v.n + kvh * a.v.h;
+  const int hd = nh % a.H, n = nh / a.H;
+  const int b0 = tile * RB, w0 = b0 + wave_id() * 32, i = w0 + (lane & 31), ic = min(i, a.L - 1);
   const float sl = a.scale * LOG2E;
   bf16x8 qf[D / 16], gf[D / 16];
   glob_frag<D>(a.q.p + n * a.q.n + (long)ic * a.q.l + hd * a.q.h, i < a.L, qf);
@@ -308,48 +432,33 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_dq_kernel(Args a) {
       for (int e = 0; e < 8; ++e)
         dd = fmaf(bf16_to_f32((unsigned short)of[s][e]), bf16_to_f32((unsigned short)gf[s][e]), dd);
   }
-  dd += __shfl_xor(dd, 32, 64);
+  dd += other_half(dd, h);
   const long row = ((long)n * a.H + hd) * a.L + ic;
-  const float lse = a.lse[row];
-  if (i < a.L && h == 0) a.dd[row] = dd;
+  const float nlse = a.lse[row];
+  if (i < a.L && h == 0) a.dd[row] = -dd;
+  const f32x16 minus_d = splat16(-dd);
   f32x16 acc[D / 32];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) acc[c] = zero16();
-  const Walk wk = key_walk(a, b0, min(b0 + RB, a.L) - 1);
-  Stage<D> sk, sv;
-  int t0 = wk.tile(0) * TK;
-  tile_load<D>(K, a.k.l, t0, a.L, sk);
-  tile_load<D>(V, a.v.l, t0, a.L, sv);
-  unsigned long long keep = tile_keep(a, n, t0);
-  tile_store<D>(kt[0], sk, keep);
-  tile_store<D>(vt[0], sv, keep);
-  __syncthreads();
-  int buf = 0;
-  for (int it = 0; it < wk.n; ++it, buf ^= 1) {
-    const int j0 = t0;
-    const unsigned long long kw = keep;
-    if (it + 1 < wk.n) {
-      t0 = wk.tile(it + 1) * TK;
-      tile_load<D>(K, a.k.l, t0, a.L, sk);
-      tile_load<D>(V, a.v.l, t0, a.L, sv);
-      keep = tile_keep(a, n, t0);
-    }
+  for (int c = 0; c < D / 32; ++c) acc[c] = splat16(0.f);
+  Frags<D> fr;
+  fr.init();
+  const Sees sees(a, w0);
+  walk_keys<D>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int jb = j0 + 32 * c;
-      const unsigned kwc = (unsigned)(kw >> (32 * c));
-      const int kind = w0 < a.L ? block_kind(a, w0, jb, kwc) : EMPTY;
+      const unsigned kw = (unsigned)(keep >> (32 * c));
+      const int kind = sees.kind(j0 + 32 * c, kw);
       if (kind == EMPTY) continue;
-      f32x16 s = zero16(), dp = zero16();
+      f32x16 s = splat16(0.f), dp = minus_d;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        s = MFMA32(row_frag<D>(kt[buf], 32 * c, t), qf[t], s);
-        dp = MFMA32(row_frag<D>(vt[buf], 32 * c, t), gf[t], dp);
+        s = MFMA32(fr.rows(k, 32 * c, t), qf[t], s);
+        dp = MFMA32(fr.rows(v, 32 * c, t), gf[t], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl, -lse)) * (dp[r] - dd);
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl, nlse)) * dp[r];
       if (kind == PARTIAL) {
-        const unsigned see = seen_keys(a, i, jb, kwc) >> (4 * h);
+        const unsigned see = seen_keys(a, i, j0 + 32 * c, kw) >> (4 * h);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = (see >> reg_bit(r)) & 1u ? s[r] : 0.f;
       }
@@ -357,15 +466,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_dq_kernel(Args a) {
       for (int t = 0; t < 2; ++t) {
         const bf16x8 b = pack8(s, t);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] = MFMA32(tr_frag<D>(kt[buf], 32 * c, t, 32 * e), b, acc[e]);
+        for (int e = 0; e < D / 32; ++e) acc[e] = MFMA32(fr.trans(k, 32 * c, t, e), b, acc[e]);
       }
     }
-    if (it + 1 < wk.n) {
-      tile_store<D>(kt[buf ^ 1], sk, keep);
-      tile_store<D>(vt[buf ^ 1], sv, keep);
-    }
-    __syncthreads();
-  }
+  });
   if (i >= a.L) return;
   unsigned short* drow = a.dq.p + n * a.dq.n + (long)i * a.dq.l + hd * a.dq.h;
 #pragma unroll
@@ -379,108 +483,116 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_dq_kernel(Args a) {
 
 // ------------------------------------------------------------------------------------ backward: dk, dv
 // Workgroup = 128 keys of one key/value head, a wave owns 32 of them; it walks the query tiles of
-// every query head of the group: P and dS (queries x keys), dv^T += dO^T P, dk^T += Q^T dS.
+// every query head of the group: P and dS (queries x keys), dv^T += dO^T P, dk^T += Q^T dS.  The rows'
+// -D are the start values of the dP accumulators, read from LDS into place.
 template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_dkv_kernel(Args a) {
-  __shared__ __attribute__((aligned(16))) unsigned short qt[2][TK * (D + 8)];
-  __shared__ __attribute__((aligned(16))) unsigned short gt[2][TK * (D + 8)];
+__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short qt[2][TK * D];
+  __shared__ __attribute__((aligned(1024))) unsigned short gt[2][TK * D];
   __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
   const int Hkv = a.H / a.G;
   const int tile = bid % a.tiles, nh = bid / a.tiles;
   const int kvh = nh % Hkv, n = nh / Hkv;
-  const int b0 = tile * RB, w0 = b0 + wave * 32, j = w0 + (lane & 31), jc = min(j, a.L - 1);
+  const int b0 = tile * RB, w0 = b0 + wave_id() * 32, j = w0 + (lane & 31), jc = min(j, a.L - 1);
   const float sl = a.scale * LOG2E;
   bool ok = j < a.L;
-  if (ok && a.mask) ok = mask_at(a, n, j) != 0;
-  const bool all_ok = (__ballot(ok) == ~0ull), any_ok = (__ballot(ok) != 0ull);
+  if (a.mask) {
+    const long mi = (long)n * a.mask_n + jc;
+    ok = ok && (a.mask_bytes == 1 ? (int)reinterpret_cast<const unsigned char*>(a.mask)[mi]
+                                  : reinterpret_cast<const int*>(a.mask)[mi]) != 0;
+  }
+  const unsigned long long okw = __ballot(ok);
+  const bool all_ok = okw == ~0ull, any_ok = okw != 0ull;
   bf16x8 kf[D / 16], vf[D / 16];
   glob_frag<D>(a.k.p + n * a.k.n + (long)jc * a.k.l + kvh * a.k.h, ok, kf);
   glob_frag<D>(a.v.p + n * a.v.n + (long)jc * a.v.l + kvh * a.v.h, ok, vf);
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = zero16();
+  for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
   // queries that see a key of this workgroup: from b0 - right to the last key + left, or to the
   // end where the workgroup holds sinks
   const int lo = max(0, b0 - a.right) / TK;
   const int last = b0 < a.sinks ? a.L - 1 : min(a.L - 1, min(b0 + RB, a.L) - 1 + a.left);
-  const int per = last / TK - lo + 1, total = per * a.G;
-  Stage<D> sq, sg;
-  float sls = 0.f, sds = 0.f;
-  auto load = [&](int it) {
-    const int hd = kvh * a.G + it / per, r0 = (lo + it % per) * TK;
-    tile_load<D>(a.q.p + n * a.q.n + hd * a.q.h, a.q.l, r0, a.L, sq);
-    tile_load<D>(a.go.p + n * a.go.n + hd * a.go.h, a.go.l, r0, a.L, sg);
-    if (threadIdx.x < TK) {
-      const long row = ((long)n * a.H + hd) * a.L + min(r0 + (int)threadIdx.x, a.L - 1);
-      sls = a.lse[row];
-      sds = a.dd[row];
+  const int per = last / TK - lo + 1, total = __syncthreads_or(any_ok) ? per * a.G : 0;
+  Frags<D> fr;
+  fr.init();
+  // the same three kinds as in the forward, seen from the wave's keys
+  const int none_lo = w0 - a.right - 31, none_hi = !any_ok ? -1 : w0 < a.sinks ? a.L - 1 : min(a.L - 1, w0 + 31 + a.left);
+  const int full_lo = w0 + 31 - a.right;
+  const int full_hi = !all_ok ? -1 : w0 + 31 < a.sinks ? a.L - 32 : min(a.L - 32, w0 + a.left - 31);
+  const int my_last = min(a.L - 1, j < a.sinks ? a.L - 1 : j + a.left);
+  Loader<D> lq, lg;
+  lq.init(a.q.l);
+  lg.init(a.go.l);
+  int hd1 = kvh * a.G, t1 = 0;  // head and tile of the tile being read
+  int buf = 1, i0t = 0;
+  operands_here();
+  for (int it = -1; it < total; ++it) {
+    const bool more = it + 1 < total;
+    const int r1 = (lo + t1) * TK;
+    if (more) {
+      lq.issue(a.q.p + n * a.q.n + hd1 * a.q.h, a.q.l, r1, a.L, qt[buf ^ 1]);
+      lg.issue(a.go.p + n * a.go.n + hd1 * a.go.h, a.go.l, r1, a.L, gt[buf ^ 1]);
+      const long row = ((long)n * a.H + hd1) * a.L;
+      if (wave_id() == 0) floats_to_lds(a.lse + row, r1, a.L, ls[buf ^ 1]);
+      if (wave_id() == 1) floats_to_lds(a.dd + row, r1, a.L, ds[buf ^ 1]);
     }
-  };
-  auto store = [&](int it, int b) {
-    const int r0 = (lo + it % per) * TK;
-    const unsigned long long keep = a.L - r0 >= 64 ? ~0ull : (1ull << (a.L - r0)) - 1ull;
-    tile_store<D>(qt[b], sq, keep);
-    tile_store<D>(gt[b], sg, keep);
-    if (threadIdx.x < TK) {
-      ls[b][threadIdx.x] = sls;
-      ds[b][threadIdx.x] = sds;
-    }
-  };
-  load(0);
-  store(0, 0);
-  __syncthreads();
-  int buf = 0;
-  for (int it = 0; it < total; ++it, buf ^= 1) {
-    const int r0 = (lo + it % per) * TK;
-    if (it + 1 < total) load(it + 1);
+    if (it >= 0) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int i0 = r0 + 32 * c;
-      // the same three kinds as in the forward, seen from the keys
-      if (!any_ok || i0 >= a.L || i0 + 31 < w0 - a.right || (i0 > w0 + 31 + a.left && w0 >= a.sinks)) continue;
-      const bool full = all_ok && i0 + 31 < a.L && i0 >= w0 + 31 - a.right &&
-                        (i0 + 31 <= w0 + a.left || w0 + 31 < a.sinks);
-      f32x16 p = zero16(), dp = zero16();
+      for (int c = 0; c < 2; ++c) {
+        const int i0 = i0t + 32 * c;
+        if (i0 < none_lo || i0 > none_hi) continue;
+        f32x16 p = splat16(0.f), dp;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) {
-        p = MFMA32(row_frag<D>(qt[buf], 32 * c, t), kf[t], p);
-        dp = MFMA32(row_frag<D>(gt[buf], 32 * c, t), vf[t], dp);
-      }
+        for (int t = 0; t < 4; ++t) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(&ds[buf][32 * c + 8 * t + 4 * h]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * c + 8 * t + 4 * h]);
-        const f32x4 dv4 = *reinterpret_cast<const f32x4*>(&ds[buf][32 * c + 8 * t + 4 * h]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * t + e;
-          p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], sl, -lv[e]));
-          dp[r] = p[r] * (dp[r] - dv4[e]);
+          for (int e = 0; e < 4; ++e) dp[4 * t + e] = d4[e];
         }
-      }
-      if (!full) {
-        const int hi = min(a.L - 1, j < a.sinks ? a.L - 1 : j + a.left);
-        const unsigned see = (ok ? bits_between(j - a.right - i0, hi - i0) : 0u) >> (4 * h);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool s = (see >> reg_bit(r)) & 1u;
-          p[r] = s ? p[r] : 0.f;
-          dp[r] = s ? dp[r] : 0.f;
+        for (int t = 0; t < D / 16; ++t) {
+          p = MFMA32(fr.rows(qt[buf], 32 * c, t), kf[t], p);
+          dp = MFMA32(fr.rows(gt[buf], 32 * c, t), vf[t], dp);
         }
-      }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const bf16x8 pb = pack8(p, t), sb = pack8(dp, t);
+        for (int t = 0; t < 4; ++t) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ls[buf][32 * c + 8 * t + 4 * h]);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          dv[e] = MFMA32(tr_frag<D>(gt[buf], 32 * c, t, 32 * e), pb, dv[e]);
-          dk[e] = MFMA32(tr_frag<D>(qt[buf], 32 * c, t, 32 * e), sb, dk[e]);
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * t + e;
+            p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], sl, l4[e]));
+            dp[r] *= p[r];
+          }
+        }
+        if (i0 < full_lo || i0 > full_hi) {
+          const unsigned see = (ok ? bits_between(j - a.right - i0, my_last - i0) : 0u) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool s = (see >> reg_bit(r)) & 1u;
+            p[r] = s ? p[r] : 0.f;
+            dp[r] = s ? dp[r] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const bf16x8 pb = pack8(p, t), sb = pack8(dp, t);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) {
+            dv[e] = MFMA32(fr.trans(gt[buf], 32 * c, t, e), pb, dv[e]);
+            dk[e] = MFMA32(fr.trans(qt[buf], 32 * c, t, e), sb, dk[e]);
+          }
         }
       }
     }
-    if (it + 1 < total) store(it + 1, buf ^ 1);
-    __syncthreads();
+    if (more) {
+      landed();
+      __syncthreads();
+      buf ^= 1;
+      i0t = r1;
+      if (++t1 == per) t1 = 0, ++hd1;
+    }
   }
   if (j >= a.L) return;
   unsigned short* kr = a.dk.p + n * a.dk.n + (long)j * a.dk.l + kvh * a.dk.h;

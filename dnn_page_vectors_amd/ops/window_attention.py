@@ -71,8 +71,9 @@ def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy of it where the kernels' 16-byte row reads could not take it."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
+    """t, or a copy of it where the kernels' 16-byte row reads or 32-bit offsets within a tile of 64 rows
+    could not take it."""
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and t.stride(1) < 1 << 24 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
