@@ -71,50 +71,56 @@ __device__ __forceinline__ constexpr int swz(int r) {
                                                  : ((r & 3) << 2) | (((r >> 2) & 1) << 1);
 }
 
+__device__ __forceinline__ unsigned lds_at(const void* p) {
+  return __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) const char*)p));
+}
+
 // Tile rows go from memory straight to LDS (global_load_lds_dwordx4: 64 lanes x 16 bytes land in 1 KB in
 // lane order), D / 32 pieces per wave; the swizzle is applied to the source column.
+// In asm: for the builtin the compiler waits for every load under way before it reads any LDS of the same array,
+// which would make the prefetch of the next tile a wait for it.  No register is written; landed() and a
+// barrier stand between these loads and the reads of their tile.
 template <int D>
 struct Loader {
   static constexpr int P = D / 32, RP = 512 / D;  // pieces per wave, rows per piece
+  static constexpr unsigned TILE = TK * D * 2;    // bytes
   unsigned off[P];                                 // this lane's source offset within a tile (bytes)
-  __device__ __forceinline__ void init(long ls) {
+  unsigned to;                                     // this wave's first piece in buffer 0
+  const char* base;                                // row 0
+  long step;                                       // bytes per row
+  __device__ __forceinline__ void init(const unsigned short* b, long ls, const unsigned short* tile) {
     const int lane = threadIdx.x & 63, w = wave_id();
+    base = reinterpret_cast<const char*>(b);
+    step = ls * 2;
+    to = lds_at(tile) + (unsigned)(w * P * 1024);
 #pragma unroll
     for (int u = 0; u < P; ++u) {
       const int r = (w * P + u) * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
       off[u] = (unsigned)(r * (int)ls + c * 8) * 2;
     }
   }
-  __device__ __forceinline__ void issue(const unsigned short* base, long ls, int r0, int L, unsigned short* t) const {
-    const int w = wave_id();
-    const unsigned short* b = base + (long)r0 * ls;
+  __device__ __forceinline__ void issue(int r0, int L, int buf) const {
+    const char* b = base + (long)r0 * step;
+    const unsigned t = to + (buf ? TILE : 0u);
     if (r0 + TK <= L) {
 #pragma unroll
-      for (int u = 0; u < P; ++u) glds(b, off[u], t + (w * P + u) * 512);
+      for (int u = 0; u < P; ++u) glds(b, off[u], t + u * 1024);
     } else {  // rows behind the sequence: its last row again (their probabilities are zero)
-      const int lane = threadIdx.x & 63;
+      const int lane = threadIdx.x & 63, w = wave_id();
 #pragma unroll
       for (int u = 0; u < P; ++u) {
         const int r = (w * P + u) * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
-        glds(b, (unsigned)(min(r, L - 1 - r0) * (int)ls + c * 8) * 2, t + (w * P + u) * 512);
+        glds(b, (unsigned)min(r, L - 1 - r0) * (unsigned)step + c * 16, t + u * 1024);
       }
     }
   }
-  // In asm: for the builtin the compiler waits for every load under way before it reads any LDS of the same array,
-  // which would make the prefetch of the next tile a wait for it.  No register is written; landed()
-  // and a barrier stand between these loads and the reads of their tile.
-  static __device__ __forceinline__ void glds(const unsigned short* base, unsigned off, unsigned short* lds) {
-    const unsigned to = __builtin_amdgcn_readfirstlane(
-        (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) unsigned short*)lds));
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to)
-                 : "memory", "m0");
+  static __device__ __forceinline__ void glds(const char* b, unsigned o, unsigned t) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(o), "s"(b), "s"(t) : "memory", "m0");
   }
 };
 
 // 64 floats x[r0 ..] of a row of L into LDS, by one wave
-__device__ __forceinline__ void floats_to_lds(const float* x, int r0, int L, float* lds) {
-  const unsigned to = __builtin_amdgcn_readfirstlane(
-      (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) float*)lds));
+__device__ __forceinline__ void floats_to_lds(const float* x, int r0, int L, unsigned to) {
   const unsigned off = (unsigned)min((int)(threadIdx.x & 63), L - 1 - r0) * 4u;
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(x + r0), "s"(to)
                : "memory", "m0");
@@ -226,8 +232,11 @@ struct Sees {
     sinks = a.sinks;
   }
   __device__ __forceinline__ int kind(int j0, unsigned kw) const {
-    if (kw == 0u || j0 > none_hi || (j0 < none_lo && j0 >= sinks)) return EMPTY;
-    return (kw == 0xFFFFFFFFu && j0 <= full_hi && (j0 >= full_lo || j0 + 32 <= sinks)) ? FULL : PARTIAL;
+    // outside / inside of an interval by the sign of the differences: a few scalar instructions, no branches
+    const int out = (none_hi - j0) | ((j0 - none_lo) & (sinks - 1 - j0));
+    const int over = (full_hi - j0) | ((j0 - full_lo) & (sinks - 32 - j0));
+    if (out < 0 || kw == 0u) return EMPTY;
+    return over >= 0 && kw == 0xFFFFFFFFu ? FULL : PARTIAL;
   }
 };
 
@@ -236,6 +245,25 @@ __device__ __forceinline__ unsigned seen_keys(const Args& a, int i, int j0, unsi
   return kw & (bits_between(i - a.left - j0, i + a.right - j0) |
                (bits_between(0, a.sinks - 1 - j0) & bits_between(0, i + a.right - j0)));
 }
+
+// Workgroup -> (sequence and head, tile).  Workgroups go to the 8 XCDs in turn: the tiles of a head stay on one XCD,
+// whose L2 then holds their keys, and heads are dealt to the XCDs one by one, so that pages of different
+// lengths spread evenly (whole ranges of sequences per XCD measured 10 % slower on ragged pages).
+struct Where {
+  int nh, tile;
+  __device__ __forceinline__ Where(int bid, int heads, int tiles) {
+    const int even = heads / 8 * 8 * tiles;
+    if (bid < even) {
+      const int i = bid / 8;
+      nh = i / tiles * 8 + bid % 8;
+      tile = i % tiles;
+    } else {
+      const int r = heads % 8, i = bid - even;
+      nh = heads - r + i % r;
+      tile = i / r;
+    }
+  }
+};
 
 // Walks the key tiles that queries b0 .. b0 + RB - 1 see (the tiles of the sinks, then the window's):
 // `each(tile K, tile V, first key, keep bits)`.  While a tile is worked on, the next one is on its way to the
@@ -248,16 +276,17 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
   const unsigned short* K = a.k.p + n * a.k.n + kvh * a.k.h;
   const unsigned short* V = a.v.p + n * a.v.n + kvh * a.v.h;
   Loader<D> lk, lv;
-  lk.init(a.k.l);
-  lv.init(a.v.l);
+  lk.init(K, a.k.l, kt[0]);
+  lv.init(V, a.v.l, vt[0]);
   const int lo = max(0, b0 - a.left) / TK, hi = min(a.L - 1, min(b0 + RB, a.L) - 1 + a.right) / TK;
   const int sink = min((a.sinks + TK - 1) / TK, lo), jump = lo - sink, tiles = sink + hi - lo + 1;
   unsigned long long some0 = 0ull, some1 = 0ull;  // tiles of this chunk of 128 that are still to come
-  int chunk = 0;                                  // first tile behind the chunk
+  int first = 0, chunk = 0;                       // its first tile, the first tile behind it
   const unsigned long long tail = a.L % TK ? (1ull << (a.L % TK)) - 1ull : ~0ull;
   const int last = (a.L - 1) / TK;
   auto refill = [&]() {
     const int m = min(tiles - chunk, 128);
+    first = chunk;
     if (a.mask) {
       __syncthreads();  // the last chunk's words have been read
       for (int t0 = 0; t0 < m; t0 += 16) {
@@ -295,8 +324,7 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
     int t = some0 ? __builtin_ctzll(some0) : 64 + __builtin_ctzll(some1);
     if (some0) some0 &= some0 - 1;
     else some1 &= some1 - 1;
-    const int base = chunk - min(chunk, ((chunk - 1) & 127) + 1);
-    const int g = base + t, tile = g < sink ? g : g + jump;
+    const int g = first + t, tile = g < sink ? g : g + jump;
     if (a.mask) {
       const unsigned long long w = words[t];
       keep = ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(w >> 32)) << 32) |
@@ -311,8 +339,8 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
   operands_here();
   while (t0 >= 0 || t1 >= 0) {  // t0: the tile worked on; t1: the tile being read
     if (t1 >= 0) {
-      lk.issue(K, a.k.l, t1 * TK, a.L, kt[buf ^ 1]);
-      lv.issue(V, a.v.l, t1 * TK, a.L, vt[buf ^ 1]);
+      lk.issue(t1 * TK, a.L, buf ^ 1);
+      lv.issue(t1 * TK, a.L, buf ^ 1);
     }
     if (t0 >= 0) each(kt[buf], vt[buf], t0 * TK, keep);
     t0 = t1;
@@ -336,10 +364,9 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short vt[2][TK * D];
   __shared__ unsigned long long words[128];
   const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile = bid % a.tiles, nh = bid / a.tiles;
-  const int hd = nh % a.H, n = nh / a.H;
-  const int b0 = tile * RB, w0 = b0 + wave_id() * 32, i = w0 + (lane & 31);
+  const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
+  const int hd = wg.nh % a.H, n = wg.nh / a.H;
+  const int b0 = wg.tile * RB, w0 = b0 + wave_id() * 32, i = w0 + (lane & 31);
   const float sl = a.scale * LOG2E, slack = fminf(SLACK / sl, 1e30f);
   bf16x8 qf[D / 16];
   glob_frag<D>(a.q.p + n * a.q.n + (long)min(i, a.L - 1) * a.q.l + hd * a.q.h, i < a.L, qf);
@@ -414,10 +441,9 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short vt[2][TK * D];
   __shared__ unsigned long long words[128];
   const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile = bid % a.tiles, nh = bid / a.tiles;
-  const int hd = nh % a.H, n = nh / a.H;
-  const int b0 = tile * RB, w0 = b0 + wave_id() * 32, i = w0 + (lane & 31), ic = min(i, a.L - 1);
+  const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
+  const int hd = wg.nh % a.H, n = wg.nh / a.H;
+  const int b0 = wg.tile * RB, w0 = b0 + wave_id() * 32, i = w0 + (lane & 31), ic = min(i, a.L - 1);
   const float sl = a.scale * LOG2E;
   bf16x8 qf[D / 16], gf[D / 16];
   glob_frag<D>(a.q.p + n * a.q.n + (long)ic * a.q.l + hd * a.q.h, i < a.L, qf);
@@ -491,11 +517,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short gt[2][TK * D];
   __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
   const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
   const int Hkv = a.H / a.G;
-  const int tile = bid % a.tiles, nh = bid / a.tiles;
-  const int kvh = nh % Hkv, n = nh / Hkv;
-  const int b0 = tile * RB, w0 = b0 + wave_id() * 32, j = w0 + (lane & 31), jc = min(j, a.L - 1);
+  const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
+  const int kvh = wg.nh % Hkv, n = wg.nh / Hkv;
+  const int b0 = wg.tile * RB, w0 = b0 + wave_id() * 32, j = w0 + (lane & 31), jc = min(j, a.L - 1);
   const float sl = a.scale * LOG2E;
   bool ok = j < a.L;
   if (a.mask) {
@@ -524,20 +549,21 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   const int full_hi = !all_ok ? -1 : w0 + 31 < a.sinks ? a.L - 32 : min(a.L - 32, w0 + a.left - 31);
   const int my_last = min(a.L - 1, j < a.sinks ? a.L - 1 : j + a.left);
   Loader<D> lq, lg;
-  lq.init(a.q.l);
-  lg.init(a.go.l);
-  int hd1 = kvh * a.G, t1 = 0;  // head and tile of the tile being read
+  lq.init(a.q.p + n * a.q.n + (long)kvh * a.G * a.q.h, a.q.l, qt[0]);
+  lg.init(a.go.p + n * a.go.n + (long)kvh * a.G * a.go.h, a.go.l, gt[0]);
+  const float *rl = a.lse + ((long)n * a.H + kvh * a.G) * a.L, *rd = a.dd + ((long)n * a.H + kvh * a.G) * a.L;
+  const unsigned ls_at = lds_at(ls[0]), ds_at = lds_at(ds[0]);
+  int t1 = 0;  // the tile being read, within its head
   int buf = 1, i0t = 0;
   operands_here();
   for (int it = -1; it < total; ++it) {
     const bool more = it + 1 < total;
     const int r1 = (lo + t1) * TK;
     if (more) {
-      lq.issue(a.q.p + n * a.q.n + hd1 * a.q.h, a.q.l, r1, a.L, qt[buf ^ 1]);
-      lg.issue(a.go.p + n * a.go.n + hd1 * a.go.h, a.go.l, r1, a.L, gt[buf ^ 1]);
-      const long row = ((long)n * a.H + hd1) * a.L;
-      if (wave_id() == 0) floats_to_lds(a.lse + row, r1, a.L, ls[buf ^ 1]);
-      if (wave_id() == 1) floats_to_lds(a.dd + row, r1, a.L, ds[buf ^ 1]);
+      lq.issue(r1, a.L, buf ^ 1);
+      lg.issue(r1, a.L, buf ^ 1);
+      if (wave_id() == 0) floats_to_lds(rl, r1, a.L, ls_at + (buf ^ 1) * TK * 4);
+      if (wave_id() == 1) floats_to_lds(rd, r1, a.L, ds_at + (buf ^ 1) * TK * 4);
     }
     if (it >= 0) {
 #pragma unroll
@@ -591,7 +617,13 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
       __syncthreads();
       buf ^= 1;
       i0t = r1;
-      if (++t1 == per) t1 = 0, ++hd1;
+      if (++t1 == per) {  // the group's next head
+        t1 = 0;
+        lq.base += a.q.h * 2;
+        lg.base += a.go.h * 2;
+        rl += a.L;
+        rd += a.L;
+      }
     }
   }
   if (j >= a.L) return;
