@@ -29,6 +29,7 @@ namespace wattn {
 constexpr int TK = 64;   // rows per staged tile
 constexpr int NTH = 256;
 constexpr int RB = 128;  // rows a workgroup owns: 4 waves x 32
+constexpr int FAR = 16;  // query tiles per workgroup of the sinks' far part
 constexpr float LOG2E = 1.4426950408889634f;
 // The running maximum is raised only when a score passes it by more than this (log2 units): until then
 // probabilities may be as large as 2^8, which costs fp32 sums and bf16 roundings nothing, and the
@@ -55,6 +56,10 @@ struct Args {
   int left, right, sinks;
   float scale;
   int tiles;  // ceil(L / RB)
+  // backward: the sinks' far queries (see bwd_dkv_kernel); far_chunks = 0: not split off
+  float* part;
+  long far_main;  // slots of the near parts
+  int far_chunks, far_blocks, far_tile;
 };
 
 #define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16((a), (b), (c), 0, 0, 0)
@@ -511,6 +516,148 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
 // Workgroup = 128 keys of one key/value head, a wave owns 32 of them; it walks the query tiles of
 // every query head of the group: P and dS (queries x keys), dv^T += dO^T P, dk^T += Q^T dS.  The rows'
 // -D are the start values of the dP accumulators, read from LDS into place.
+//
+// The sinks are seen by every later query: walked by their own workgroup alone they would make it the last
+// by far.  Their far queries (behind the window's tiles) are dealt to workgroups of FAR tiles each, whose
+// waves share 32 keys and split the queries; partial sums in fp32, added up by sink_sum_kernel.
+template <int D>
+struct KeyGrads {
+  bf16x8 kf[D / 16], vf[D / 16];
+  f32x16 dk[D / 32], dv[D / 32];
+  // 32 queries (rows r0 .. of the tiles, ls / ds their -log-sum-exp and -D) against the wave's 32 keys
+  __device__ __forceinline__ void block(const Frags<D>& fr, const unsigned short* qt, const unsigned short* gt, int r0,
+                                        const float* ls, const float* ds, float sl, unsigned see, bool full) {
+    const int h = (threadIdx.x & 63) >> 5;
+    f32x16 p = splat16(0.f), dp;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(ds + 8 * t + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * t + e] = d4[e];
+    }
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      p = MFMA32(fr.rows(qt, r0, t), kf[t], p);
+      dp = MFMA32(fr.rows(gt, r0, t), vf[t], dp);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 8 * t + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * t + e;
+        p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], sl, l4[e]));
+        dp[r] *= p[r];
+      }
+    }
+    if (!full) {
+      see >>= 4 * h;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool s = (see >> reg_bit(r)) & 1u;
+        p[r] = s ? p[r] : 0.f;
+        dp[r] = s ? dp[r] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bf16x8 pb = pack8(p, t), sb = pack8(dp, t);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) {
+        dv[e] = MFMA32(fr.trans(gt, r0, t, e), pb, dv[e]);
+        dk[e] = MFMA32(fr.trans(qt, r0, t, e), sb, dk[e]);
+      }
+    }
+  }
+};
+
+// the keys of a partial row set: [dk, dv][d][32 keys] fp32
+template <int D>
+__device__ __forceinline__ float* part_at(float* part, long slot, int which, int e, int r) {
+  const int lane = threadIdx.x & 63;
+  return part + ((slot * 2 + which) * D + 32 * e + reg_bit(r) + 4 * (lane >> 5)) * 32 + (lane & 31);
+}
+
+// the wave's 32 keys w0 ..: whether this lane's counts, K and V in registers, sums cleared
+template <int D>
+__device__ __forceinline__ bool key_lane(const Args& a, int n, int kvh, int j, KeyGrads<D>& w) {
+  const int jc = min(j, a.L - 1);
+  bool ok = j < a.L;
+  if (a.mask) {
+    const long mi = (long)n * a.mask_n + jc;
+    ok = ok && (a.mask_bytes == 1 ? (int)reinterpret_cast<const unsigned char*>(a.mask)[mi]
+                                  : reinterpret_cast<const int*>(a.mask)[mi]) != 0;
+  }
+  glob_frag<D>(a.k.p + n * a.k.n + (long)jc * a.k.l + kvh * a.k.h, ok, w.kf);
+  glob_frag<D>(a.v.p + n * a.v.n + (long)jc * a.v.l + kvh * a.v.h, ok, w.vf);
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) w.dk[c] = w.dv[c] = splat16(0.f);
+  return ok;
+}
+
+template <int D>
+__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_far_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short tiles[4][TK * D];  // Q, Q, dO, dO
+  __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
+  const int lane = threadIdx.x & 63, wv = wave_id();
+  int x = blockIdx.x;  // (sequence, head), 32-key block of sinks, chunk of query tiles
+  const int ch = x % a.far_chunks;
+  x /= a.far_chunks;
+  const int kb = x % a.far_blocks;
+  x /= a.far_blocks;
+  const int hd = x % a.H, n = x / a.H, w0 = kb * 32, j = w0 + (lane & 31);
+  const float sl = a.scale * LOG2E;
+  KeyGrads<D> w;
+  const bool ok = key_lane<D>(a, n, hd / a.G, j, w);
+  const unsigned long long okw = __ballot(ok);
+  Frags<D> fr;
+  fr.init();
+  Loader<D> lq, lg;
+  lq.init(a.q.p + n * a.q.n + (long)hd * a.q.h, a.q.l, tiles[0]);
+  lg.init(a.go.p + n * a.go.n + (long)hd * a.go.h, a.go.l, tiles[2]);
+  const float *rl = a.lse + ((long)n * a.H + hd) * a.L, *rd = a.dd + ((long)n * a.H + hd) * a.L;
+  const unsigned ls_at = lds_at(ls[0]), ds_at = lds_at(ds[0]);
+  const int t0 = a.far_tile + ch * FAR, t1 = min(t0 + FAR, (a.L + TK - 1) / TK);
+  if (okw != 0ull)
+    for (int t = t0; t < t1; t += 2) {  // two tiles at a time, one 32-row block per wave
+      const int n2 = min(2, t1 - t);
+      for (int u = 0; u < n2; ++u) {
+        lq.issue((t + u) * TK, a.L, u);
+        lg.issue((t + u) * TK, a.L, u);
+        if (wv == 0) floats_to_lds(rl, (t + u) * TK, a.L, ls_at + u * TK * 4);
+        if (wv == 1) floats_to_lds(rd, (t + u) * TK, a.L, ds_at + u * TK * 4);
+      }
+      landed();
+      __syncthreads();
+      const int u = wv >> 1, r0 = 32 * (wv & 1), i0 = (t + u) * TK + r0;
+      if (u < n2 && i0 < a.L) {
+        const unsigned see = ok && j < a.sinks ? bits_between(0, a.L - 1 - i0) : 0u;
+        w.block(fr, tiles[u], tiles[2 + u], r0, &ls[u][r0], &ds[u][r0], sl, see,
+                okw == ~0ull && w0 + 32 <= a.sinks && i0 + 32 <= a.L);
+      }
+      __syncthreads();
+    }
+  // the four waves' sums, added in wave order
+  float* red = reinterpret_cast<float*>(&tiles[0][0]);  // 4 x 1024 floats
+  static_assert(sizeof(tiles) >= 4 * 1024 * sizeof(float), "the waves' sums fit the tiles' place");
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) red[wv * 1024 + r * 64 + lane] = which ? w.dv[e][r] : w.dk[e][r];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = 4 * wv + q;
+        float y = red[r * 64 + lane];
+#pragma unroll
+        for (int v = 1; v < 4; ++v) y += red[v * 1024 + r * 64 + lane];
+        part_at<D>(a.part, a.far_main + blockIdx.x, which, e, 0)[(8 * wv + q) * 32] = y;  // its row: 8 wv + q + 4 h
+      }
+    }
+}
+
 template <int D>
 __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short qt[2][TK * D];
@@ -520,34 +667,25 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   const int Hkv = a.H / a.G;
   const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
   const int kvh = wg.nh % Hkv, n = wg.nh / Hkv;
-  const int b0 = wg.tile * RB, w0 = b0 + wave_id() * 32, j = w0 + (lane & 31), jc = min(j, a.L - 1);
+  const int b0 = wg.tile * RB, w0 = b0 + wave_id() * 32, j = w0 + (lane & 31);
   const float sl = a.scale * LOG2E;
-  bool ok = j < a.L;
-  if (a.mask) {
-    const long mi = (long)n * a.mask_n + jc;
-    ok = ok && (a.mask_bytes == 1 ? (int)reinterpret_cast<const unsigned char*>(a.mask)[mi]
-                                  : reinterpret_cast<const int*>(a.mask)[mi]) != 0;
-  }
+  const bool split = a.far_chunks != 0;
+  KeyGrads<D> w;
+  const bool ok = key_lane<D>(a, n, kvh, j, w);
   const unsigned long long okw = __ballot(ok);
   const bool all_ok = okw == ~0ull, any_ok = okw != 0ull;
-  bf16x8 kf[D / 16], vf[D / 16];
-  glob_frag<D>(a.k.p + n * a.k.n + (long)jc * a.k.l + kvh * a.k.h, ok, kf);
-  glob_frag<D>(a.v.p + n * a.v.n + (long)jc * a.v.l + kvh * a.v.h, ok, vf);
-  f32x16 dk[D / 32], dv[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
-  // queries that see a key of this workgroup: from b0 - right to the last key + left, or to the
-  // end where the workgroup holds sinks
+  // queries that see a key of this workgroup: from b0 - right to the last key + left, or (sinks
+  // that are not split off) to the end
   const int lo = max(0, b0 - a.right) / TK;
-  const int last = b0 < a.sinks ? a.L - 1 : min(a.L - 1, min(b0 + RB, a.L) - 1 + a.left);
+  const int last = b0 < a.sinks && !split ? a.L - 1 : min(a.L - 1, min(b0 + RB, a.L) - 1 + a.left);
   const int per = last / TK - lo + 1, total = __syncthreads_or(any_ok) ? per * a.G : 0;
-  Frags<D> fr;
-  fr.init();
   // the same three kinds as in the forward, seen from the wave's keys
   const int none_lo = w0 - a.right - 31, none_hi = !any_ok ? -1 : w0 < a.sinks ? a.L - 1 : min(a.L - 1, w0 + 31 + a.left);
   const int full_lo = w0 + 31 - a.right;
   const int full_hi = !all_ok ? -1 : w0 + 31 < a.sinks ? a.L - 32 : min(a.L - 32, w0 + a.left - 31);
   const int my_last = min(a.L - 1, j < a.sinks ? a.L - 1 : j + a.left);
+  Frags<D> fr;
+  fr.init();
   Loader<D> lq, lg;
   lq.init(a.q.p + n * a.q.n + (long)kvh * a.G * a.q.h, a.q.l, qt[0]);
   lg.init(a.go.p + n * a.go.n + (long)kvh * a.G * a.go.h, a.go.l, gt[0]);
@@ -570,46 +708,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
       for (int c = 0; c < 2; ++c) {
         const int i0 = i0t + 32 * c;
         if (i0 < none_lo || i0 > none_hi) continue;
-        f32x16 p = splat16(0.f), dp;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(&ds[buf][32 * c + 8 * t + 4 * h]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dp[4 * t + e] = d4[e];
-        }
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-          p = MFMA32(fr.rows(qt[buf], 32 * c, t), kf[t], p);
-          dp = MFMA32(fr.rows(gt[buf], 32 * c, t), vf[t], dp);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ls[buf][32 * c + 8 * t + 4 * h]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * t + e;
-            p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], sl, l4[e]));
-            dp[r] *= p[r];
-          }
-        }
-        if (i0 < full_lo || i0 > full_hi) {
-          const unsigned see = (ok ? bits_between(j - a.right - i0, my_last - i0) : 0u) >> (4 * h);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool s = (see >> reg_bit(r)) & 1u;
-            p[r] = s ? p[r] : 0.f;
-            dp[r] = s ? dp[r] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bf16x8 pb = pack8(p, t), sb = pack8(dp, t);
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) {
-            dv[e] = MFMA32(fr.trans(gt[buf], 32 * c, t, e), pb, dv[e]);
-            dk[e] = MFMA32(fr.trans(qt[buf], 32 * c, t, e), sb, dk[e]);
-          }
-        }
+        const bool full = i0 >= full_lo && i0 <= full_hi;
+        unsigned see = 0u;
+        if (!full) see = ok ? bits_between(j - a.right - i0, my_last - i0) : 0u;
+        w.block(fr, qt[buf], gt[buf], 32 * c, &ls[buf][32 * c], &ds[buf][32 * c], sl, see, full);
       }
     }
     if (more) {
@@ -626,7 +728,17 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
       }
     }
   }
-  if (j >= a.L) return;
+  if (split && w0 < a.sinks) {  // the sinks' near part: added to the far ones, every key of the block
+    const long slot = ((long)n * Hkv + kvh) * a.far_blocks + w0 / 32;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        *part_at<D>(a.part, slot, 0, e, r) = w.dk[e][r];
+        *part_at<D>(a.part, slot, 1, e, r) = w.dv[e][r];
+      }
+  }
+  if (j >= a.L || (split && j < a.sinks)) return;
   unsigned short* kr = a.dk.p + n * a.dk.n + (long)j * a.dk.l + kvh * a.dk.h;
   unsigned short* vr = a.dv.p + n * a.dv.n + (long)j * a.dv.l + kvh * a.dv.h;
 #pragma unroll
@@ -634,11 +746,31 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       *reinterpret_cast<uint2*>(kr + e * 32 + 8 * t + 4 * h) =
-          uint2{pack_bf16x2(dk[e][4 * t] * a.scale, dk[e][4 * t + 1] * a.scale),
-                pack_bf16x2(dk[e][4 * t + 2] * a.scale, dk[e][4 * t + 3] * a.scale)};
+          uint2{pack_bf16x2(w.dk[e][4 * t] * a.scale, w.dk[e][4 * t + 1] * a.scale),
+                pack_bf16x2(w.dk[e][4 * t + 2] * a.scale, w.dk[e][4 * t + 3] * a.scale)};
       *reinterpret_cast<uint2*>(vr + e * 32 + 8 * t + 4 * h) =
-          uint2{pack_bf16x2(dv[e][4 * t], dv[e][4 * t + 1]), pack_bf16x2(dv[e][4 * t + 2], dv[e][4 * t + 3])};
+          uint2{pack_bf16x2(w.dv[e][4 * t], w.dv[e][4 * t + 1]), pack_bf16x2(w.dv[e][4 * t + 2], w.dv[e][4 * t + 3])};
     }
+}
+
+// dk, dv of the sinks: near part + the group's heads' chunks, in that order.  Grid (N Hkv, blocks of 32 keys).
+__global__ __launch_bounds__(256) void sink_sum_kernel(Args a, int D) {
+  const int Hkv = a.H / a.G, kvh = blockIdx.x % Hkv, n = blockIdx.x / Hkv, kb = blockIdx.y;
+  const int key = threadIdx.x & 31, j = kb * 32 + key, rows = 2 * D;
+  if (j >= a.sinks) return;
+  const long set = (long)rows * 32;
+  const float* near = a.part + (((long)n * Hkv + kvh) * a.far_blocks + kb) * set;
+  for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+    float x = near[r * 32 + key];
+    for (int g = 0; g < a.G; ++g) {
+      const float* far =
+          a.part + (a.far_main + (((long)n * a.H + kvh * a.G + g) * a.far_blocks + kb) * a.far_chunks) * set + r * 32 + key;
+#pragma unroll 4
+      for (int c = 0; c < a.far_chunks; ++c) x += far[c * set];
+    }
+    const View& o = r < D ? a.dk : a.dv;
+    o.p[n * o.n + (long)j * o.l + kvh * o.h + (r < D ? r : r - D)] = f32_to_bf16(r < D ? x * a.scale : x);
+  }
 }
 
 #undef MFMA32
@@ -655,6 +787,29 @@ __host__ inline int check_sizes(long N, long L, long H, long G, int d, float sca
   if (L > (1L << 29) || !(scale > 0.f)) return -3;
   const long blocks = (L + RB - 1) / RB * H * N;
   return blocks > 0x7FFFFFFFL ? -4 : 0;
+}
+
+// The far part of the sinks is split off where they all lie in the first workgroup of keys and it is long
+// enough to matter (8 tiles: a window's own walk at left + right = 384).  More sinks than that fill several
+// workgroups with long walks, which balance among themselves.
+struct FarPlan {
+  int wgs, chunks, blocks, tile;
+  long near_slots, floats;
+};
+__host__ inline FarPlan far_plan(long N, long L, long H, long G, int d, int left, int sinks) {
+  FarPlan f{};
+  const long l = left < L ? left : L, tiles = (L + TK - 1) / TK;
+  const long first = (RB - 1 + l < L - 1 ? RB - 1 + l : L - 1) / TK + 1;
+  if (sinks <= 0 || sinks > RB || tiles - first < 8) return f;
+  f.tile = (int)first;
+  f.chunks = (int)((tiles - first + FAR - 1) / FAR);
+  f.blocks = (sinks + 31) / 32;
+  const long wgs = N * H * f.blocks * f.chunks;
+  if (wgs > (1L << 30)) return FarPlan{};
+  f.wgs = (int)wgs;
+  f.near_slots = N * (H / G) * f.blocks;
+  f.floats = (f.near_slots + wgs) * 2 * d * 32;
+  return f;
 }
 
 }  // namespace wattn
@@ -698,11 +853,17 @@ PV_API int pv_wattn_fwd(const void* q, const void* k, const void* v, void* o, co
   return 0;
 }
 
-// st: strides of q, k, v, o, go, dq, dk, dv.  dd (N, H, L) fp32 workspace; dq (N, L, H, d), dk, dv
+// floats of workspace that pv_wattn_bwd needs besides dd
+PV_API long pv_wattn_bwd_ws(int N, int L, int H, int G, int d, int left, int sinks) {
+  return N > 0 && L > 0 && H > 0 && G > 0 ? far_plan(N, L, H, G, d, left, min(sinks, L)).floats : 0;
+}
+
+// st: strides of q, k, v, o, go, dq, dk, dv.  dd (N, H, L) and ws fp32 workspace; dq (N, L, H, d), dk, dv
 // (N, L, H / G, d) bf16, every element written.
 PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const void* go, void* dq, void* dk,
                         void* dv, const long* st, const void* mask, long mask_n, int mask_bytes, float* lse, float* dd,
-                        int N, int L, int H, int G, int d, int left, int right, int sinks, float scale, void* stream) {
+                        float* ws, long ws_floats, int N, int L, int H, int G, int d, int left, int right, int sinks,
+                        float scale, void* stream) {
   if (const int rc = check_sizes(N, L, H, G, d, scale)) return rc;
   Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, L, H, G, left, right, sinks, scale);
   a.go = view(go, st, 4);
@@ -710,12 +871,20 @@ PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void*
   a.dk = view(dk, st, 6);
   a.dv = view(dv, st, 7);
   a.dd = dd;
+  const FarPlan f = far_plan(N, L, H, G, d, a.left, a.sinks);
+  if (f.floats > 0 && (!ws || ws_floats < f.floats)) return -5;
+  a.part = ws;
+  a.far_chunks = f.chunks;
+  a.far_blocks = f.blocks;
+  a.far_tile = f.tile;
+  a.far_main = f.near_slots;
   const dim3 gq((unsigned)((long)a.tiles * H * N)), gk((unsigned)((long)a.tiles * (H / G) * N));
   hipStream_t s = (hipStream_t)stream;
 #define PV_WBWD(DV)                                                 \
   do {                                                              \
     hipLaunchKernelGGL(bwd_dq_kernel<DV>, gq, dim3(NTH), 0, s, a);  \
     PV_LAUNCH_CHECK();                                              \
+    if (f.wgs) hipLaunchKernelGGL(bwd_far_kernel<DV>, dim3(f.wgs), dim3(NTH), 0, s, a); \
     hipLaunchKernelGGL(bwd_dkv_kernel<DV>, gk, dim3(NTH), 0, s, a); \
     PV_LAUNCH_CHECK();                                              \
   } while (0)
@@ -723,5 +892,9 @@ PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void*
   else if (d == 64) PV_WBWD(64);
   else PV_WBWD(128);
 #undef PV_WBWD
+  if (f.wgs) {
+    hipLaunchKernelGGL(sink_sum_kernel, dim3((unsigned)(N * (H / G)), f.blocks), dim3(256), 0, s, a, d);
+    PV_LAUNCH_CHECK();
+  }
   return 0;
 }

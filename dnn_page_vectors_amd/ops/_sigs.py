@@ -136,7 +136,8 @@ SIGS = {
     "pv_scale": "p" "lf" "p",
     # window_attention.hip
     "pv_wattn_fwd": "ppppp" "pli" "p" "iiiii" "iii" "f" "p",
-    "pv_wattn_bwd": "ppppp" "pppp" "pli" "pp" "iiiii" "iii" "f" "p",
+    "pv_wattn_bwd_ws": "iiiii" "ii",
+    "pv_wattn_bwd": "ppppp" "pppp" "pli" "pp" "pl" "iiiii" "iii" "f" "p",
     # token_embedding.hip
     "pv_temb_fwd": "pipipi" "lli" "f" "pp" "ppi" "p",
     "pv_temb_grad_ws": "lli",
@@ -160,7 +161,7 @@ SIGS = {
 
 _RESTYPE = {"pv_rsort_temp_bytes": ctypes.c_long, "pv_ib_fwd_dq_parts": ctypes.c_long, "pv_ib_bwd_ws": ctypes.c_long, "pv_ib_fwd_ws": ctypes.c_long,
             "pv_bias_gelu_bwd_ws": ctypes.c_long, "pv_layernorm_bwd_ws": ctypes.c_long,
-            "pv_ibw_ws": ctypes.c_long, "pv_temb_grad_ws": ctypes.c_long, "pv_ckpt8_gelu_bwd_ws": ctypes.c_long}
+            "pv_ibw_ws": ctypes.c_long, "pv_wattn_bwd_ws": ctypes.c_long, "pv_temb_grad_ws": ctypes.c_long, "pv_ckpt8_gelu_bwd_ws": ctypes.c_long}
 
 
 def declare(lib) -> None:

@@ -96,11 +96,14 @@ def _forward(q, k, v, out, mask, win, scale: float, lse) -> None:
 
 def _backward(q, k, v, out, do, dq, dk, dv, mask, win, scale: float, lse) -> None:
     N, L, H, d = q.shape
+    G = H // k.shape[2]
     D = torch.empty_like(lse)
+    n = lib().pv_wattn_bwd_ws(N, L, H, G, d, win[0], win[2]) if win[2] else 0
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     st = _strides(q, k, v, out, do, dq, dk, dv)
     with on_device(q):
         check(lib().pv_wattn_bwd(P(q), P(k), P(v), P(out), P(do), P(dq), P(dk), P(dv), st, *_mask_args(mask), P(lse),
-                                 P(D), N, L, H, H // k.shape[2], d, *win, scale, stream(q.device)), "pv_wattn_bwd")
+                                 P(D), P(ws), n, N, L, H, G, d, *win, scale, stream(q.device)), "pv_wattn_bwd")
 
 
 class _WindowAttnFn(torch.autograd.Function):

@@ -239,6 +239,19 @@ def test_long_sinks_and_wide_scores():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("L,left,right,sinks", [(1100, 20, 20, 1), (1000, 5, 0, 40), (1217, 64, 3, 128), (2300, 10, 10, 33),
+                                                (1700, 0, 0, 32), (1000, 20, 20, 129)])
+def test_far_queries_of_the_sinks(d, L, left, right, sinks):
+    """Sinks seen from far behind their window: summed by workgroups of their own."""
+    check(*inputs(1, L, 2, 1, d, L), left, right, sinks, None)
+    if d == 64:
+        m = ragged(3, L, 2, holes=True)
+        m[1, :7] = False                     # a masked sink
+        check(*inputs(3, L, 2, 2, d, L + 1), left, right, sinks, m)
+
+
+@pytest.mark.gpu
 def test_strides():
     N, L, H, d = 2, 130, 3, 64
     g = torch.Generator().manual_seed(0)
