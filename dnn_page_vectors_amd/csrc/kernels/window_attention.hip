@@ -29,7 +29,7 @@ namespace wattn {
 constexpr int TK = 64;   // rows per staged tile
 constexpr int NTH = 256;
 constexpr int RB = 128;  // rows a workgroup owns: 4 waves x 32
-constexpr int FAR = 16;  // query tiles per workgroup of the sinks' far part
+constexpr int FAR = 4;   // query tiles per workgroup of the sinks' far part
 constexpr float LOG2E = 1.4426950408889634f;
 // The running maximum is raised only when a score passes it by more than this (log2 units): until then
 // probabilities may be as large as 2^8, which costs fp32 sums and bf16 roundings nothing, and the
@@ -88,34 +88,37 @@ __device__ __forceinline__ unsigned lds_at(const void* p) {
 template <int D>
 struct Loader {
   static constexpr int P = D / 32, RP = 512 / D;  // pieces per wave, rows per piece
-  static constexpr unsigned TILE = TK * D * 2;    // bytes
-  unsigned off[P];                                 // this lane's source offset within a tile (bytes)
-  unsigned to;                                     // this wave's first piece in buffer 0
-  const char* base;                                // row 0
-  long step;                                       // bytes per row
+  static constexpr int KINDS = RP % 8 ? 2 : 1;     // swz repeats every 8 rows: pieces of 4 rows come in two kinds
+  static constexpr unsigned TILE = TK * D * 2;     // bytes
+  unsigned off[KINDS];                              // this lane's source offset within a piece (bytes)
+  unsigned to;                                      // this wave's first piece in buffer 0
+  const char* base;                                 // row 0
+  long step;                                        // bytes per row
   __device__ __forceinline__ void init(const unsigned short* b, long ls, const unsigned short* tile) {
-    const int lane = threadIdx.x & 63, w = wave_id();
+    const int lane = threadIdx.x & 63;
     base = reinterpret_cast<const char*>(b);
     step = ls * 2;
-    to = lds_at(tile) + (unsigned)(w * P * 1024);
+    to = lds_at(tile) + (unsigned)(wave_id() * P * 1024);
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const int r = (w * P + u) * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
-      off[u] = (unsigned)(r * (int)ls + c * 8) * 2;
+    for (int k = 0; k < KINDS; ++k) {
+      const int r = lane / (D / 8);
+      off[k] = (unsigned)(r * (int)step) + (unsigned)(((lane % (D / 8)) ^ swz<D>(r + RP * k)) * 16);
     }
   }
   __device__ __forceinline__ void issue(int r0, int L, int buf) const {
-    const char* b = base + (long)r0 * step;
     const unsigned t = to + (buf ? TILE : 0u);
+    const int w0 = r0 + wave_id() * P * RP;  // this wave's first row
+    const char* b = base + (long)w0 * step;
     if (r0 + TK <= L) {
 #pragma unroll
-      for (int u = 0; u < P; ++u) glds(b, off[u], t + u * 1024);
+      for (int u = 0; u < P; ++u) glds(b + (long)(u * RP) * step, off[u % KINDS], t + u * 1024);
     } else {  // rows behind the sequence: its last row again (their probabilities are zero)
-      const int lane = threadIdx.x & 63, w = wave_id();
+      const int lane = threadIdx.x & 63;
+      const char* b0 = base + (long)r0 * step;
 #pragma unroll
       for (int u = 0; u < P; ++u) {
-        const int r = (w * P + u) * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
-        glds(b, (unsigned)min(r, L - 1 - r0) * (unsigned)step + c * 16, t + u * 1024);
+        const int r = (w0 - r0) + u * RP + lane / (D / 8), c = (lane % (D / 8)) ^ swz<D>(r);
+        glds(b0, (unsigned)min(r, L - 1 - r0) * (unsigned)step + c * 16, t + u * 1024);
       }
     }
   }
@@ -157,28 +160,23 @@ __device__ __forceinline__ void clear_rows(unsigned short* k, unsigned short* v,
 // This lane's addresses within a tile.  A operand of a product: rows (lane & 31), columns 16 s + 8 (lane / 32).
 // Transposed A operand: row = tile column (lane & 31) of a 32-column group; its 8 k-slots are the tile rows
 // that registers 8 s .. 8 s + 7 of a 32 x 32 accumulator hold in this half-wave: 16 s + 4 h + {0..3}, +8.
+// The swizzle touches other address bits than the row and the tile do, so a step in columns is an exclusive or
+// with a constant: one register for each kind of address.
 template <int D>
 struct Frags {
-  unsigned row[D / 16], tr[D / 32];  // bytes
+  unsigned row, tr;  // bytes
   __device__ __forceinline__ void init() {
     const int lane = threadIdx.x & 63, h = lane >> 5, g = lane >> 4;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const int r = lane & 31;
-      row[s] = (unsigned)(r * D * 2 + ((2 * s + h) ^ swz<D>(r)) * 16);
-    }
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      const int r = 4 * (g >> 1) + ((lane & 15) >> 2), c = 32 * e + 16 * (g & 1) + 4 * (lane & 3);
-      tr[e] = (unsigned)(r * D * 2 + ((c >> 3) ^ swz<D>(r)) * 16 + (c & 7) * 2);
-    }
+    row = (unsigned)((lane & 31) * D * 2 + (h ^ swz<D>(lane & 31)) * 16);
+    const int r = 4 * (g >> 1) + ((lane & 15) >> 2), c = 16 * (g & 1) + 4 * (lane & 3);
+    tr = (unsigned)(r * D * 2 + ((c >> 3) ^ swz<D>(r)) * 16 + (c & 7) * 2);
   }
   // rows r0 .. r0 + 31 (r0 a multiple of 32; swz repeats every 8 rows)
   __device__ __forceinline__ bf16x8 rows(const unsigned short* t, int r0, int s) const {
-    return *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(t) + row[s] + r0 * D * 2);
+    return *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(t) + (row ^ (32u * s)) + r0 * D * 2);
   }
   __device__ __forceinline__ bf16x8 trans(const unsigned short* t, int r0, int s, int e) const {
-    const char* p = reinterpret_cast<const char*>(t) + tr[e] + (r0 + 16 * s) * D * 2;
+    const char* p = reinterpret_cast<const char*>(t) + (tr ^ (64u * e)) + (r0 + 16 * s) * D * 2;
     const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
     const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 8 * D * 2));
     return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -571,11 +569,11 @@ struct KeyGrads {
   }
 };
 
-// the keys of a partial row set: [dk, dv][d][32 keys] fp32
+// Partial sums of the sinks, fp32: slots of [dk, dv][sink][D].  Lane's four values of accumulator quad t of column
+// group e: d = 32 e + 8 t + 4 h ..
 template <int D>
-__device__ __forceinline__ float* part_at(float* part, long slot, int which, int e, int r) {
-  const int lane = threadIdx.x & 63;
-  return part + ((slot * 2 + which) * D + 32 * e + reg_bit(r) + 4 * (lane >> 5)) * 32 + (lane & 31);
+__device__ __forceinline__ float* part_at(const Args& a, long slot, int which, int key, int e, int t) {
+  return a.part + ((slot * 2 + which) * a.sinks + key) * D + 32 * e + 8 * t + 4 * ((threadIdx.x & 63) >> 5);
 }
 
 // the wave's 32 keys w0 ..: whether this lane's counts, K and V in registers, sums cleared
@@ -596,16 +594,14 @@ __device__ __forceinline__ bool key_lane(const Args& a, int n, int kvh, int j, K
 }
 
 template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_far_kernel(Args a) {
+__global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_far_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short tiles[4][TK * D];  // Q, Q, dO, dO
   __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
   const int lane = threadIdx.x & 63, wv = wave_id();
-  int x = blockIdx.x;  // (sequence, head), 32-key block of sinks, chunk of query tiles
-  const int ch = x % a.far_chunks;
-  x /= a.far_chunks;
-  const int kb = x % a.far_blocks;
-  x /= a.far_blocks;
-  const int hd = x % a.H, n = x / a.H, w0 = kb * 32, j = w0 + (lane & 31);
+  // ((sequence, head), chunk of query tiles), 32-key block of sinks
+  const int kb = blockIdx.x % a.far_blocks, slot = blockIdx.x / a.far_blocks;
+  const int ch = slot % a.far_chunks, nh = slot / a.far_chunks;
+  const int hd = nh % a.H, n = nh / a.H, w0 = kb * 32, j = w0 + (lane & 31);
   const float sl = a.scale * LOG2E;
   KeyGrads<D> w;
   const bool ok = key_lane<D>(a, n, hd / a.G, j, w);
@@ -637,25 +633,28 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_far_kernel(Args a) {
       }
       __syncthreads();
     }
-  // the four waves' sums, added in wave order
+  // the four waves' sums, added in wave order; wave wv finishes accumulator quad wv
   float* red = reinterpret_cast<float*>(&tiles[0][0]);  // 4 x 1024 floats
   static_assert(sizeof(tiles) >= 4 * 1024 * sizeof(float), "the waves' sums fit the tiles' place");
-  for (int which = 0; which < 2; ++which)
+  auto finish = [&](const f32x16& x, int which, int e) {
+    __syncthreads();
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      __syncthreads();
+    for (int r = 0; r < 16; ++r) red[wv * 1024 + r * 64 + lane] = x[r];
+    __syncthreads();
+    f32x4 y;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) red[wv * 1024 + r * 64 + lane] = which ? w.dv[e][r] : w.dk[e][r];
-      __syncthreads();
+    for (int q = 0; q < 4; ++q) {
+      y[q] = red[(4 * wv + q) * 64 + lane];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = 4 * wv + q;
-        float y = red[r * 64 + lane];
-#pragma unroll
-        for (int v = 1; v < 4; ++v) y += red[v * 1024 + r * 64 + lane];
-        part_at<D>(a.part, a.far_main + blockIdx.x, which, e, 0)[(8 * wv + q) * 32] = y;  // its row: 8 wv + q + 4 h
-      }
+      for (int v = 1; v < 4; ++v) y[q] += red[v * 1024 + (4 * wv + q) * 64 + lane];
     }
+    if (j < a.sinks) *reinterpret_cast<f32x4*>(part_at<D>(a, a.far_main + slot, which, j, e, wv)) = y;
+  };
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) {
+    finish(w.dk[e], 0, e);
+    finish(w.dv[e], 1, e);
+  }
 }
 
 template <int D>
@@ -728,14 +727,16 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
       }
     }
   }
-  if (split && w0 < a.sinks) {  // the sinks' near part: added to the far ones, every key of the block
-    const long slot = ((long)n * Hkv + kvh) * a.far_blocks + w0 / 32;
+  if (split && j < a.sinks) {  // the sinks' near part: added to the far ones
 #pragma unroll
     for (int e = 0; e < D / 32; ++e)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        *part_at<D>(a.part, slot, 0, e, r) = w.dk[e][r];
-        *part_at<D>(a.part, slot, 1, e, r) = w.dv[e][r];
+      for (int t = 0; t < 4; ++t) {
+        f32x4 x, y;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = w.dk[e][4 * t + q], y[q] = w.dv[e][4 * t + q];
+        *reinterpret_cast<f32x4*>(part_at<D>(a, (long)n * Hkv + kvh, 0, j, e, t)) = x;
+        *reinterpret_cast<f32x4*>(part_at<D>(a, (long)n * Hkv + kvh, 1, j, e, t)) = y;
       }
   }
   if (j >= a.L || (split && j < a.sinks)) return;
@@ -753,24 +754,22 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
     }
 }
 
-// dk, dv of the sinks: near part + the group's heads' chunks, in that order.  Grid (N Hkv, blocks of 32 keys).
-__global__ __launch_bounds__(256) void sink_sum_kernel(Args a, int D) {
-  const int Hkv = a.H / a.G, kvh = blockIdx.x % Hkv, n = blockIdx.x / Hkv, kb = blockIdx.y;
-  const int key = threadIdx.x & 31, j = kb * 32 + key, rows = 2 * D;
-  if (j >= a.sinks) return;
-  const long set = (long)rows * 32;
-  const float* near = a.part + (((long)n * Hkv + kvh) * a.far_blocks + kb) * set;
-  for (int r = threadIdx.x >> 5; r < rows; r += 8) {
-    float x = near[r * 32 + key];
-    for (int g = 0; g < a.G; ++g) {
-      const float* far =
-          a.part + (a.far_main + (((long)n * a.H + kvh * a.G + g) * a.far_blocks + kb) * a.far_chunks) * set + r * 32 + key;
-#pragma unroll 4
-      for (int c = 0; c < a.far_chunks; ++c) x += far[c * set];
-    }
-    const View& o = r < D ? a.dk : a.dv;
-    o.p[n * o.n + (long)j * o.l + kvh * o.h + (r < D ? r : r - D)] = f32_to_bf16(r < D ? x * a.scale : x);
+// dk, dv of the sinks: near part + the group's heads' chunks, in that order.  Thread = element of a slot
+// (2 x sinks x D), grid.y = sequence and key/value head.
+__global__ __launch_bounds__(64) void sink_sum_kernel(Args a, int D) {
+  const int Hkv = a.H / a.G, kvh = blockIdx.y % Hkv, n = blockIdx.y / Hkv;
+  const int x = blockIdx.x * 64 + threadIdx.x, half = a.sinks * D;
+  if (x >= 2 * half) return;
+  const long set = 2L * half;
+  float y = a.part[((long)n * Hkv + kvh) * set + x];
+  for (int g = 0; g < a.G; ++g) {
+    const float* far = a.part + (a.far_main + ((long)n * a.H + kvh * a.G + g) * a.far_chunks) * set + x;
+#pragma unroll 8
+    for (int c = 0; c < a.far_chunks; ++c) y += far[c * set];
   }
+  const int which = x >= half, i = which ? x - half : x, j = i / D, d = i - j * D;
+  const View& o = which ? a.dv : a.dk;
+  o.p[n * o.n + (long)j * o.l + kvh * o.h + d] = f32_to_bf16(which ? y : y * a.scale);
 }
 
 #undef MFMA32
@@ -800,15 +799,15 @@ __host__ inline FarPlan far_plan(long N, long L, long H, long G, int d, int left
   FarPlan f{};
   const long l = left < L ? left : L, tiles = (L + TK - 1) / TK;
   const long first = (RB - 1 + l < L - 1 ? RB - 1 + l : L - 1) / TK + 1;
-  if (sinks <= 0 || sinks > RB || tiles - first < 8) return f;
+  if (sinks <= 0 || sinks > RB || tiles - first < 8 || N * (H / G) > 65535) return f;
   f.tile = (int)first;
   f.chunks = (int)((tiles - first + FAR - 1) / FAR);
   f.blocks = (sinks + 31) / 32;
   const long wgs = N * H * f.blocks * f.chunks;
   if (wgs > (1L << 30)) return FarPlan{};
   f.wgs = (int)wgs;
-  f.near_slots = N * (H / G) * f.blocks;
-  f.floats = (f.near_slots + wgs) * 2 * d * 32;
+  f.near_slots = N * (H / G);
+  f.floats = (f.near_slots + N * H * f.chunks) * 2 * d * sinks;
   return f;
 }
 
@@ -893,7 +892,7 @@ PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void*
   else PV_WBWD(128);
 #undef PV_WBWD
   if (f.wgs) {
-    hipLaunchKernelGGL(sink_sum_kernel, dim3((unsigned)(N * (H / G)), f.blocks), dim3(256), 0, s, a, d);
+    hipLaunchKernelGGL(sink_sum_kernel, dim3((2 * a.sinks * d + 63) / 64, (unsigned)(N * (H / G))), dim3(64), 0, s, a, d);
     PV_LAUNCH_CHECK();
   }
   return 0;
