@@ -73,95 +73,99 @@ __device__ __forceinline__ void store8(unsigned short* p, const float (&x)[8]) {
 }
 
 // ------------------------------------------------------------------------------------ lookup
-// A workgroup owns `rows` consecutive tokens; a thread takes pieces of C columns of them (C = 8: 16-byte
-// stores; C = 1: row lengths or pointers that are no multiple of 16 bytes).
+// A workgroup owns `rows` consecutive tokens; a thread takes pieces of C columns of them, four at a time so that
+// four rows are on their way at once (C = 8: 16-byte stores; C = 1: row lengths or pointers that are no
+// multiple of 16 bytes).
 template <typename TW, typename TO, int C>
 __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restrict__ W, TO* __restrict__ out, long T,
                                                      long V, int E, float scale, int rows,
                                                      const float* __restrict__ pos, const float* __restrict__ typ,
                                                      Groups gr) {
   const long t0 = (long)blockIdx.x * rows;
-  const int n = (int)min((long)rows, T - t0), per = E / C;
-  for (int x = threadIdx.x; x < n * per; x += 256) {
-    const int r = x / per, c = (x - r * per) * C;
-    const long t = t0 + r;
-    const long id = ids.at(t);
-    const bool ok = id >= 0 && id < V;
-    float v[C];
-    if constexpr (C == 8) load8(W + (ok ? id : 0) * E + c, v);
-    else v[0] = load1(W + (ok ? id : 0) * E + c);
+  const int n = (int)min((long)rows, T - t0), per = E / C, all = n * per;
+  for (int x0 = threadIdx.x; x0 < all; x0 += 1024) {
+    int r[4], c[4];
+    long id[4];
+    float v[4][C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = ok ? v[i] * scale : __uint_as_float(0x7FC00000u);
-    if (pos) {
-      int g = 0;
-      while (g + 1 < gr.n && t >= gr.off[g + 1]) ++g;
-      const float* pp = pos + (size_t)((t - gr.off[g]) % gr.L[g]) * E + c;
-#pragma unroll
-      for (int i = 0; i < C; ++i) v[i] = (v[i] + pp[i]) + typ[c + i];
+    for (int u = 0; u < 4; ++u) {
+      const int x = min(x0 + 256 * u, all - 1);
+      r[u] = x / per;
+      c[u] = (x - r[u] * per) * C;
+      id[u] = ids.at(t0 + r[u]);
     }
-    if constexpr (C == 8) store8(out + t * E + c, v);
-    else store1(out + t * E + c, v[0]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const TW* w = W + (id[u] >= 0 && id[u] < V ? id[u] : 0) * E + c[u];
+      if constexpr (C == 8) load8(w, v[u]);
+      else v[u][0] = load1(w);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (x0 + 256 * u >= all) break;
+      const long t = t0 + r[u];
+      const bool ok = id[u] >= 0 && id[u] < V;
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[u][i] = ok ? v[u][i] * scale : __uint_as_float(0x7FC00000u);
+      if (pos) {
+        int g = 0;
+        while (g + 1 < gr.n && t >= gr.off[g + 1]) ++g;
+        const float* pp = pos + (size_t)((t - gr.off[g]) % gr.L[g]) * E + c[u];
+#pragma unroll
+        for (int i = 0; i < C; ++i) v[u][i] = (v[u][i] + pp[i]) + typ[c[u] + i];
+      }
+      if constexpr (C == 8) store8(out + t * E + c[u], v[u]);
+      else store1(out + t * E + c[u], v[u][0]);
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------ gradient
-// A lane owns W consecutive columns (4, or 1 where rows are not 4-aligned) of NJ column groups of a
-// slab of 64 W NJ columns.
-template <typename TG, int W, int NJ>
+// A lane owns W consecutive columns (4, or 1 where rows are not 4-aligned) of a slab of 64 W columns (grid.y).
+// One slab per wave: a wave over a whole row of 768 has a third of the waves and as many loads under way
+// (walk_kernel 87 us instead of 44 at 73728 tokens x 768).
+template <typename TG, int W>
 struct Cols {
-  float a[NJ][W];
+  float a[W];
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < W; ++i) a[j][i] = 0.f;
+    for (int i = 0; i < W; ++i) a[i] = 0.f;
   }
-  __device__ __forceinline__ static int col(int j) {
-    return blockIdx.y * (64 * W * NJ) + j * 64 * W + (threadIdx.x & 63) * W;
-  }
+  __device__ __forceinline__ static int col() { return (blockIdx.y * 64 + (threadIdx.x & 63)) * W; }
   __device__ __forceinline__ void load(const TG* row, int E) {
+    const int c = col();
+    if (c >= E) {
+      zero();
+    } else if constexpr (W == 1) {
+      a[0] = load1(row + c);
+    } else if constexpr (sizeof(TG) == 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(row + c);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int c = col(j);
-      if (c >= E) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) a[j][i] = 0.f;
-      } else if constexpr (W == 1) {
-        a[j][0] = load1(row + c);
-      } else if constexpr (sizeof(TG) == 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(row + c);
-#pragma unroll
-        for (int i = 0; i < W; ++i) a[j][i] = v[i];
-      } else {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(row + c);
-        a[j][0] = __uint_as_float(v[0] << 16);
-        a[j][1] = __uint_as_float(v[0] & 0xFFFF0000u);
-        a[j][2] = __uint_as_float(v[1] << 16);
-        a[j][3] = __uint_as_float(v[1] & 0xFFFF0000u);
-      }
+      for (int i = 0; i < W; ++i) a[i] = v[i];
+    } else {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(row + c);
+      a[0] = __uint_as_float(v[0] << 16);
+      a[1] = __uint_as_float(v[0] & 0xFFFF0000u);
+      a[2] = __uint_as_float(v[1] << 16);
+      a[3] = __uint_as_float(v[1] & 0xFFFF0000u);
     }
   }
   template <typename O>
   __device__ __forceinline__ void add(const O& x) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < W; ++i) a[j][i] += x.a[j][i];
+    for (int i = 0; i < W; ++i) a[i] += x.a[i];
   }
   // dst row = (acc ? dst row : 0) + scale * this
   __device__ __forceinline__ void store(float* row, int E, float scale, bool acc) const {
+    const int c = col();
+    if (c >= E) return;
+    if constexpr (W == 1) {
+      row[c] = (acc ? row[c] : 0.f) + a[0] * scale;
+    } else {
+      f32x4 v = acc ? *reinterpret_cast<const f32x4*>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int c = col(j);
-      if (c >= E) continue;
-      if constexpr (W == 1) {
-        row[c] = (acc ? row[c] : 0.f) + a[j][0] * scale;
-      } else {
-        f32x4 v = acc ? *reinterpret_cast<const f32x4*>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] += a[j][i] * scale;
-        *reinterpret_cast<f32x4*>(row + c) = v;
-      }
+      for (int i = 0; i < W; ++i) v[i] += a[i] * scale;
+      *reinterpret_cast<f32x4*>(row + c) = v;
     }
   }
 };
@@ -169,33 +173,29 @@ struct Cols {
 __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Sum over the four waves of a workgroup in wave order, into wave 0's x
-template <typename X, int W, int NJ>
-__device__ __forceinline__ void join_waves(X& x, float (&sh)[3][NJ][W][64]) {
+template <typename X, int W>
+__device__ __forceinline__ void join_waves(X& x, float (&sh)[3][W][64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (wave)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < W; ++i) sh[wave - 1][j][i][lane] = x.a[j][i];
+    for (int i = 0; i < W; ++i) sh[wave - 1][i][lane] = x.a[i];
   __syncthreads();
   if (wave == 0)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int w = 0; w < 3; ++w) x.a[j][i] += sh[w][j][i][lane];
+      for (int w = 0; w < 3; ++w) x.a[i] += sh[w][i][lane];
 }
 
 // Few tokens.  Workgroup b < T: token b, which writes its id's row if it is the id's first token
 // (every wave adds the rows of one quarter of the tokens).  Workgroups behind: zeros for the rows
 // without a token.
-template <typename TG, int W, int NJ>
+template <typename TG, int W>
 __global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __restrict__ g, float* __restrict__ dW,
                                                          int T, long V, int E, long pad, float scale, int acc) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x < T) {
-    __shared__ float sh[3][NJ][W][64];
+    __shared__ float sh[3][W][64];
     const int t = blockIdx.x;
     const unsigned v = ids.key(t, V, pad);
     if (v == (unsigned)V) return;
@@ -203,18 +203,26 @@ __global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __re
     for (int u = threadIdx.x; u < t; u += 256) before |= ids.key(u, V, pad) == v;
     if (__syncthreads_or(before)) return;
     const int q = (T - t + 3) / 4, u0 = t + wave * q, u1 = min(T, u0 + q);
-    Cols<TG, W, NJ> sum, row;
+    Cols<TG, W> sum;
     sum.zero();
     for (int u = u0; u < u1; u += 64) {
       unsigned long long hit = __ballot(u + lane < u1 && ids.key(min(u + lane, T - 1), V, pad) == v);
-      while (hit) {
-        const int k = __builtin_ctzll(hit);
-        hit &= hit - 1;
-        row.load(g + (size_t)(u + k) * E, E);
-        sum.add(row);
+      while (hit) {  // four rows on their way at once, added in token order
+        Cols<TG, W> row[4];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = hit ? __builtin_ctzll(hit) : 0;
+          n += hit != 0ull;
+          row[i].load(g + (size_t)(u + k) * E, E);
+          hit &= hit - 1;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) sum.add(row[i]);
       }
     }
-    join_waves<Cols<TG, W, NJ>, W, NJ>(sum, sh);
+    join_waves<Cols<TG, W>, W>(sum, sh);
     if (wave == 0) sum.store(dW + (size_t)v * E, E, scale, acc);
     return;
   }
@@ -255,7 +263,7 @@ __global__ __launch_bounds__(256) void key_kernel(Ids ids, KT* __restrict__ keys
 // A wave adds the rows of its chunk of the sorted tokens, run by run.  Partial rows: slot 2 c = the
 // part of a run that began before chunk c, slot 2 c + 1 = the part of a run that begins in chunk c
 // and goes on behind it.
-template <typename TG, typename KT, int W, int NJ>
+template <typename TG, typename KT, int W>
 __global__ __launch_bounds__(256) void walk_kernel(const KT* __restrict__ keys, const unsigned* __restrict__ slot,
                                                    const TG* __restrict__ g, float* __restrict__ part,
                                                    float* __restrict__ dW, long T, long V, int E, float scale,
@@ -274,7 +282,7 @@ __global__ __launch_bounds__(256) void walk_kernel(const KT* __restrict__ keys, 
   const bool from_before = b > 0 && keys[b - 1] == (KT)cur;
   const unsigned behind = e < T ? (unsigned)keys[e] : none;
   bool first = true;
-  Cols<TG, W, NJ> sum;
+  Cols<TG, W> sum;
   sum.zero();
   auto flush = [&](unsigned key, bool goes_on) {
     if (first && from_before) sum.store(part + (2 * c) * E, E, 1.f, false);
@@ -284,9 +292,9 @@ __global__ __launch_bounds__(256) void walk_kernel(const KT* __restrict__ keys, 
     sum.zero();
   };
   const int n = (int)(e - b);
-  constexpr int U = NJ >= 4 ? 4 : 8;  // rows in flight
+  constexpr int U = 8;  // rows on their way at once (16: 103 instead of 83 us at 256000 tokens x 512)
   for (int k0 = 0; k0 < n; k0 += U) {
-    Cols<TG, W, NJ> row[U];
+    Cols<TG, W> row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const unsigned p = __builtin_amdgcn_readlane(mypos, min(k0 + u, n - 1));
@@ -307,36 +315,54 @@ __global__ __launch_bounds__(256) void walk_kernel(const KT* __restrict__ keys, 
   flush(cur, behind == cur);
 }
 
-// A workgroup per chunk: where a run begins in chunk c and goes on behind it, the sum of its partial
-// rows (each wave adds one quarter of them).
-template <typename TG, typename KT, int W, int NJ>
+// Where a run begins in chunk c and goes on behind it: the sum of its partial rows.  A wave per chunk; runs over
+// many chunks (frequent ids) are added by the workgroup's four waves together, a quarter each.
+constexpr int ALONE = 16;  // partial rows that a wave adds by itself
+template <typename TG, typename KT, int W>
 __global__ __launch_bounds__(256) void join_kernel(const KT* __restrict__ keys, const float* __restrict__ part,
                                                    float* __restrict__ dW, long T, long V, int E, float scale,
                                                    int acc) {
-  __shared__ float sh[3][NJ][W][64];
-  const long c = blockIdx.x, b = c * CHUNK, e = b + CHUNK;
-  if (e >= T) return;
-  const KT key = keys[e - 1];
-  if ((unsigned)key == (unsigned)V || keys[e] != key) return;
-  if (keys[b] == key && b > 0 && keys[b - 1] == key) return;  // began before this chunk
-  long lo = e, hi = T;  // first position behind the run
-  while (lo < hi) {
-    const long mid = (lo + hi) >> 1;
-    if (keys[mid] == key) lo = mid + 1;
-    else hi = mid;
-  }
-  const long m = (lo - 1) / CHUNK - c + 1;  // partial rows: slot 2c+1, then 2(c+1), 2(c+2), ..
+  __shared__ float sh[3][W][64];
+  __shared__ long many[4];
   const int wave = threadIdx.x >> 6;
-  const long q = (m + 3) / 4, x0 = wave * q, x1 = min(m, x0 + q);
-  Cols<float, W, NJ> sum, row;
-  sum.zero();
-#pragma unroll 4
-  for (long x = x0; x < x1; ++x) {
-    row.load(part + (x == 0 ? 2 * c + 1 : 2 * (c + x)) * E, E);
-    sum.add(row);
+  auto total = [&](long c, long x0, long x1) {  // partial rows x0 .. of the run that begins in chunk c
+    Cols<float, W> sum, row;
+    sum.zero();
+#pragma unroll 8
+    for (long x = x0; x < x1; ++x) {
+      row.load(part + (x == 0 ? 2 * c + 1 : 2 * (c + x)) * E, E);
+      sum.add(row);
+    }
+    return sum;
+  };
+  {
+    const long c = (long)blockIdx.x * 4 + wave, b = c * CHUNK, e = b + CHUNK;
+    long m = 0;
+    if (e < T) {
+      const KT key = keys[e - 1];
+      if ((unsigned)key != (unsigned)V && keys[e] == key && !(keys[b] == key && b > 0 && keys[b - 1] == key)) {
+        long lo = e, hi = T;  // first position behind the run
+        while (lo < hi) {
+          const long mid = (lo + hi) >> 1;
+          if (keys[mid] == key) lo = mid + 1;
+          else hi = mid;
+        }
+        m = (lo - 1) / CHUNK - c + 1;  // slot 2c+1, then 2(c+1), 2(c+2), ..
+        if (m <= ALONE) total(c, 0, m).store(dW + (size_t)key * E, E, scale, acc);
+      }
+    }
+    if ((threadIdx.x & 63) == 0) many[wave] = m > ALONE ? m : 0;
   }
-  join_waves<Cols<float, W, NJ>, W, NJ>(sum, sh);
-  if (wave == 0) sum.store(dW + (size_t)key * E, E, scale, acc);
+  __syncthreads();
+  for (int w = 0; w < 4; ++w) {
+    const long m = many[w], c = (long)blockIdx.x * 4 + w;
+    if (!m) continue;
+    const long q = (m + 3) / 4, x0 = wave * q;
+    Cols<float, W> sum = total(c, x0, min(m, x0 + q));
+    join_waves<Cols<float, W>, W>(sum, sh);
+    if (wave == 0) sum.store(dW + (size_t)keys[c * CHUNK + CHUNK - 1] * E, E, scale, acc);
+    __syncthreads();
+  }
 }
 
 __host__ inline size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -368,7 +394,7 @@ __host__ inline Layout layout(long T, long V, int E) {
   return l;
 }
 
-template <typename TG, typename KT, int W, int NJ>
+template <typename TG, typename KT, int W>
 int sorted_grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc,
                 char* ws, const Layout& l, hipStream_t st) {
   KT *keys = (KT*)(ws + l.keys), *sk = (KT*)(ws + l.skeys);
@@ -379,51 +405,41 @@ int sorted_grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, l
   hipLaunchKernelGGL((key_kernel<KT>), dim3((unsigned)min(want, 4096L)), dim3(256), 0, st, ids, keys, T, V, pad, dW, z);
   PV_LAUNCH_CHECK();
   if (const int rc = pv_rsort_pairs(ws + l.temp, l.temp_bytes, keys, sk, nullptr, slot, T, l.bits, l.kb, st)) return rc;
-  const int slabs = (E + 64 * W * NJ - 1) / (64 * W * NJ);
-  hipLaunchKernelGGL((walk_kernel<TG, KT, W, NJ>), dim3((unsigned)((l.chunks + 3) / 4), slabs), dim3(256), 0, st,
+  const int slabs = (E + 64 * W - 1) / (64 * W);
+  hipLaunchKernelGGL((walk_kernel<TG, KT, W>), dim3((unsigned)((l.chunks + 3) / 4), slabs), dim3(256), 0, st,
                      (const KT*)sk, (const unsigned*)slot, g, part, dW, T, V, E, scale, acc);
   PV_LAUNCH_CHECK();
-  hipLaunchKernelGGL((join_kernel<TG, KT, W, NJ>), dim3((unsigned)l.chunks, slabs), dim3(256), 0, st, (const KT*)sk,
+  hipLaunchKernelGGL((join_kernel<TG, KT, W>), dim3((unsigned)((l.chunks + 3) / 4), slabs), dim3(256), 0, st, (const KT*)sk,
                      (const float*)part, dW, T, V, E, scale, acc);
   PV_LAUNCH_CHECK();
   return 0;
 }
 
-template <typename TG, int W, int NJ>
+template <typename TG, int W>
 int grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
          long ws_bytes, hipStream_t st) {
   if (T <= SMALL_T) {
-    const int slabs = (E + 64 * W * NJ - 1) / (64 * W * NJ);
+    const int slabs = (E + 64 * W - 1) / (64 * W);
     const long z = acc ? 0 : (V + ZROWS - 1) / ZROWS;
     if (T + z > 0x7FFFFFFFL) return -4;
     if (T + z == 0) return 0;
-    hipLaunchKernelGGL((small_grad_kernel<TG, W, NJ>), dim3((unsigned)(T + z), slabs), dim3(256), 0, st, ids, g, dW,
+    hipLaunchKernelGGL((small_grad_kernel<TG, W>), dim3((unsigned)(T + z), slabs), dim3(256), 0, st, ids, g, dW,
                        (int)T, V, E, pad, scale, acc);
     PV_LAUNCH_CHECK();
     return 0;
   }
   const Layout l = layout(T, V, E);
   if (!ws || (size_t)ws_bytes < l.bytes) return -5;
-  return l.kb == 2 ? sorted_grad<TG, unsigned short, W, NJ>(ids, g, dW, T, V, E, pad, scale, acc, ws, l, st)
-                   : sorted_grad<TG, unsigned, W, NJ>(ids, g, dW, T, V, E, pad, scale, acc, ws, l, st);
-}
-
-template <typename TG, int W>
-int grad_nj(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
-            long ws_bytes, hipStream_t st) {
-  const int groups = (E + 64 * W - 1) / (64 * W);
-  if (groups == 1) return grad<TG, W, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
-  if (groups == 2) return grad<TG, W, 2>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
-  if (groups == 3) return grad<TG, W, 3>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
-  return grad<TG, W, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+  return l.kb == 2 ? sorted_grad<TG, unsigned short, W>(ids, g, dW, T, V, E, pad, scale, acc, ws, l, st)
+                   : sorted_grad<TG, unsigned, W>(ids, g, dW, T, V, E, pad, scale, acc, ws, l, st);
 }
 
 template <typename TG>
 int grad_w(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
            long ws_bytes, hipStream_t st) {
   const bool vec = E % 4 == 0 && ((size_t)g % (4 * sizeof(TG))) == 0 && ((size_t)dW % 16) == 0;
-  return vec ? grad_nj<TG, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st)
-             : grad_nj<TG, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+  return vec ? grad<TG, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st)
+             : grad<TG, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
 }
 
 template <typename TW, typename TO>
