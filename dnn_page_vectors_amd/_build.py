@@ -1,4 +1,4 @@
-"""In-tree native build: HIP kernels (hipcc, gfx950) + C++ host runtime (g++).
+"""In-tree native build: HIP kernels (hipcc, gfx950), the C++ autograd binding and the C++ host runtime (g++).
 
 Outputs go to ``dnn_page_vectors_amd/lib/`` so they travel with the repo
 snapshot to the GPU box (``*.so`` is git-ignored, not gpurun-ignored).
@@ -27,6 +27,7 @@ OBJ = os.path.join(PKG, "lib", "obj")
 HIP_LIB = os.path.join(LIB, "libpagevec_hip.so")
 HIP_DEBUG_LIB = os.path.join(LIB, "libpagevec_hip_debug.so")  # PV_CHECK preconditions compiled in
 RT_LIB = os.path.join(LIB, "libpagevec_rt.so")
+TORCH_LIB = os.path.join(LIB, "pagevec_torch.so")  # Python module: autograd nodes over the kernels' launchers
 
 ARCH = os.environ.get("PAGEVEC_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -139,7 +140,7 @@ def _link(objs: List[str], out: str, linker: List[str], verbose: bool) -> bool:
     if os.path.exists(out) and os.path.exists(stamp) and open(stamp).read() == key:
         return False
     tmp = out + ".tmp"
-    _run(linker + ["-shared", "-o", tmp] + objs, verbose)
+    _run(linker[:1] + objs + linker[1:] + ["-shared", "-o", tmp], verbose)  # libraries behind the objects
     os.replace(tmp, out)
     with open(stamp, "w") as f:
         f.write(key)
@@ -188,9 +189,47 @@ def _build_hip(verbose: bool = False, jobs: int = 4, debug: bool = False) -> str
     return out
 
 
+def _binding_inputs():
+    """Sources, flags and linker arguments of the autograd binding (against the installed torch)."""
+    import importlib.util
+    import sysconfig
+
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        version = f.read()
+    rocm = os.path.dirname(os.path.dirname(HIPCC))
+    inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(rocm, "include")]
+    # the torch version in the flags: another torch is another object
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-DPV_TORCH_{hashlib.sha1(version.encode()).hexdigest()[:12]}"] + [x for d in inc for x in ("-isystem", d)]
+    link = [CXX, "-L" + os.path.join(torch_dir, "lib"), "-Wl,--no-as-needed", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            "-lc10", "-lc10_hip"]
+    return _sources(os.path.join(CSRC, "binding"), ".cpp"), flags, os.path.join(CSRC, "binding"), link
+
+
+def binding_stale() -> bool:
+    """True when the autograd binding is missing or was built from other sources or for another torch."""
+    stamp = TORCH_LIB + ".stamp"
+    if not (os.path.exists(TORCH_LIB) and os.path.exists(stamp)):
+        return True
+    srcs, flags, incdir, _ = _binding_inputs()
+    with open(stamp) as f:
+        return f.read().strip() != _stamp_of(_objects(srcs, CXX, flags, incdir, "bind"))
+
+
+def build_binding(verbose: bool = False, jobs: int = 4) -> str:
+    with _BuildLock():
+        srcs, flags, incdir, link = _binding_inputs()
+        objs = _compile_all(srcs, CXX, flags, incdir, "bind", jobs, verbose)
+        _link(objs, TORCH_LIB, link, verbose)
+    return TORCH_LIB
+
+
 def build_all(verbose: bool = False, jobs: int = 0) -> None:
     jobs = jobs or min(8, os.cpu_count() or 4)
     build_runtime(verbose, jobs)
+    build_binding(verbose, jobs)
     build_hip(verbose, jobs)
 
 
@@ -213,6 +252,7 @@ def main(argv: Sequence[str] = ()) -> None:
     if a.hip or not a.rt:
         if not a.hip:
             build_runtime(a.verbose, jobs)
+            build_binding(a.verbose, jobs)
         build_hip(a.verbose, jobs)
     elif a.rt:
         build_runtime(a.verbose, jobs)

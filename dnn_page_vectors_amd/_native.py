@@ -1,7 +1,8 @@
-"""ctypes loaders for the two in-tree native libraries.
+"""Loaders for the in-tree native libraries.
 
 * ``libpagevec_rt.so``  — C++ host runtime (featurizer, JSONL reader). CPU only.
 * ``libpagevec_hip.so`` — hand-written HIP/CDNA4 kernels (gfx950).
+* ``pagevec_torch.so``  — autograd nodes of the latency-bound operators in C++, over the kernels' launchers.
 
 Policy: on a machine with a GPU the HIP library is *required* — ops raise
 ``NativeUnavailable`` instead of silently falling back to PyTorch.  The pure
@@ -177,13 +178,45 @@ def hip(required: bool = True) -> Optional[ctypes.CDLL]:
     return _hip
 
 
+_binding = None
+_binding_for: Optional[ctypes.CDLL] = None
+_BINDING_NEEDS = ("pv_wattn_fwd", "pv_wattn_bwd_ws", "pv_wattn_bwd", "pv_temb_fwd", "pv_temb_grad_ws", "pv_temb_grad",
+                  "pv_ckpt8_pack", "pv_ckpt8_unpack", "pv_ckpt8_gelu_fwd", "pv_ckpt8_gelu_bwd_ws", "pv_ckpt8_gelu_bwd")
+
+
+def binding():
+    """The C++ autograd module, calling the launchers of the kernel library in use (required on a GPU)."""
+    global _binding, _binding_for
+    lib = hip(required=True)
+    if _binding is not None and _binding_for is lib:
+        return _binding
+    with _lock:
+        if _binding is None:
+            import importlib.machinery
+            import importlib.util
+
+            if _build.binding_stale():
+                if not _autobuild():
+                    raise NativeUnavailable(f"{_build.TORCH_LIB} is missing or stale; run python -m dnn_page_vectors_amd._build")
+                _build.build_binding()
+            loader = importlib.machinery.ExtensionFileLoader("pagevec_torch", _build.TORCH_LIB)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("pagevec_torch", _build.TORCH_LIB,
+                                                                                            loader=loader))
+            loader.exec_module(module)
+            _binding = module
+        if _binding_for is not lib:
+            _binding.init({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _BINDING_NEEDS})
+            _binding_for = lib
+    return _binding
+
+
 def loaded_libraries() -> list:
     """Paths of in-tree native libraries mapped into this process (for smoke checks)."""
     out = []
     try:
         with open("/proc/self/maps") as f:
             for line in f:
-                if "libpagevec_" in line:
+                if "libpagevec_" in line or "pagevec_torch" in line:
                     p = line.split()[-1]
                     if p not in out:
                         out.append(p)

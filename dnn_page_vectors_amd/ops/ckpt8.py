@@ -21,6 +21,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from .. import _native
 from . import dense as dops
 from . import grad_sink
 from . import transformer as tops
@@ -89,13 +90,7 @@ def pack(x: torch.Tensor) -> Packed:
     x = x.detach()
     if not use_hip(x):
         return Packed(*_pack_reference(x), x.dtype)
-    x = x.contiguous()
-    q, s = _alloc(x)
-    D = x.shape[-1]
-    with on_device(x):
-        check(lib().pv_ckpt8_pack(P(x), int(x.dtype == torch.bfloat16), P(q), P(s), x.numel() // D, D,
-                                  stream(x.device)), "pv_ckpt8_pack")
-    return Packed(q, s, x.dtype)
+    return Packed(*_native.binding().pack(x), x.dtype)
 
 
 def unpack(p: Packed, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -110,12 +105,7 @@ def unpack(p: Packed, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         raise ValueError("ckpt8.unpack: values and scales are on different devices")
     if not use_hip(p.q):
         return _unpack_reference(p.q, p.s).to(dtype)
-    q, s = p.q.contiguous(), p.s.contiguous()
-    x = torch.empty(q.shape, dtype=dtype, device=q.device)
-    with on_device(q):
-        check(lib().pv_ckpt8_unpack(P(q), P(s), P(x), int(dtype == torch.bfloat16), q.numel() // D, D,
-                                    stream(q.device)), "pv_ckpt8_unpack")
-    return x
+    return _native.binding().unpack(p.q, p.s, dtype == torch.bfloat16)
 
 
 # ---- bias + GELU -----------------------------------------------------------------------------------------
@@ -179,6 +169,9 @@ def _bias_ok(x: torch.Tensor, b: torch.Tensor, name: str) -> None:
 
 
 class _BiasGelu8Fn(torch.autograd.Function):
+    """CPU, and biases whose gradient lives in the flat buffer (ops/optim.py::FlatParams): the kernel adds into it.  Other
+    biases on the GPU take the C++ node (csrc/binding/autograd.cpp)."""
+
     @staticmethod
     def forward(ctx, x, b):
         y, p = gelu_pack(x.contiguous(), b.float().contiguous())
@@ -204,6 +197,8 @@ def bias_gelu(x: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     _bias_ok(x, b, "ckpt8.bias_gelu")
     if not (torch.is_grad_enabled() and (x.requires_grad or b.requires_grad)):
         return tops.bias_gelu(x, b)  # nothing to keep
+    if use_hip(x) and grad_sink.flat_of(b) is None:
+        return _native.binding().bias_gelu8(x, b)
     return _BiasGelu8Fn.apply(x, b)
 
 

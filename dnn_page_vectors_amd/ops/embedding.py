@@ -24,6 +24,7 @@ from typing import Optional
 
 import torch
 
+from .. import _native
 from . import dense as dops
 from . import grad_sink
 from . import reference as ref
@@ -479,6 +480,9 @@ def sorted_row_grad(ids: torch.Tensor, g: torch.Tensor, dst: torch.Tensor, scale
 
 
 class _ScaledEmbeddingFn(torch.autograd.Function):
+    """scaled_embedding of a parameter whose gradient lives in the flat buffer (ops/optim.py::FlatParams): the kernel
+    adds into it.  Other tables take the C++ node (csrc/binding/autograd.cpp)."""
+
     @staticmethod
     def forward(ctx, W, ids, scale, padding_idx, out_dtype):
         out = torch.empty(ids.numel(), W.shape[1], dtype=out_dtype, device=W.device)
@@ -536,8 +540,7 @@ def scaled_embedding(ids: torch.Tensor, W: torch.Tensor, scale: float = 1.0, pad
     if W.shape[1] == 0 or V == 0 or ids.numel() >= 1 << 31 or V >= (1 << 31) - 1 or W.shape[1] > 1 << 20:
         raise ValueError(f"scaled_embedding: {ids.numel()} tokens of a {tuple(W.shape)} table are outside the kernels' range")
     ids = ids.contiguous()
-    if torch.is_grad_enabled() and W.requires_grad:
+    if torch.is_grad_enabled() and W.requires_grad and grad_sink.flat_of(W) is not None:
         return _ScaledEmbeddingFn.apply(W, ids, float(scale), padding_idx, out_dtype)
-    out = torch.empty(*ids.shape, W.shape[1], dtype=out_dtype, device=W.device)
-    lookup_rows(ids, W.detach().contiguous(), out.view(-1, W.shape[1]), scale)
-    return out
+    return _native.binding().scaled_embedding(W, ids, float(scale), -1 if padding_idx is None else int(padding_idx),
+                                              out_dtype == torch.bfloat16)

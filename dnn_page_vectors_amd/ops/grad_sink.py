@@ -40,6 +40,11 @@ def _flat(p: torch.Tensor):
     return getattr(p, "_pv_flat", None) if ENABLED else None
 
 
+def flat_of(p: torch.Tensor):
+    """The FlatParams that p's gradient is a view of, or None."""
+    return _flat(p)
+
+
 def accum_target(p: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if p is None or torch.is_grad_enabled():  # create_graph backward: keep autograd's path
         return None

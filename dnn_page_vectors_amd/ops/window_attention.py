@@ -18,6 +18,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
+from .. import _native
 from ._common import P, check, lib, on_device, stream, use_hip
 
 HEAD_DIMS = (32, 64, 128)
@@ -70,14 +71,6 @@ def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         raise ValueError("window_attention: q, k, v are on different devices")
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy of it where the kernels' 16-byte row reads or 32-bit offsets within a tile of 64 rows
-    could not take it."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and t.stride(1) < 1 << 24 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
-
-
 def _strides(*ts: torch.Tensor):
     return (ctypes.c_long * (3 * len(ts)))(*[s for t in ts for s in t.stride()[:3]])
 
@@ -85,6 +78,8 @@ def _strides(*ts: torch.Tensor):
 def _mask_args(mask: Optional[torch.Tensor]):
     return (None, 0, 1) if mask is None else (mask.data_ptr(), mask.stride(0), mask.element_size())
 
+
+# the packed form's calls (views of one buffer); the plain form's are in csrc/binding/autograd.cpp
 
 def _forward(q, k, v, out, mask, win, scale: float, lse) -> None:
     N, L, H, d = q.shape
@@ -104,31 +99,6 @@ def _backward(q, k, v, out, do, dq, dk, dv, mask, win, scale: float, lse) -> Non
     with on_device(q):
         check(lib().pv_wattn_bwd(P(q), P(k), P(v), P(out), P(do), P(dq), P(dk), P(dv), st, *_mask_args(mask), P(lse),
                                  P(D), P(ws), n, N, L, H, G, d, *win, scale, stream(q.device)), "pv_wattn_bwd")
-
-
-class _WindowAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, mask, win, scale):
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        N, L, H, d = q.shape
-        out = torch.empty(N, L, H, d, dtype=q.dtype, device=q.device)
-        lse = torch.empty(N, H, L, dtype=torch.float32, device=q.device)
-        _forward(q, k, v, out, mask, win, scale, lse)
-        ctx.save_for_backward(q, k, v, out, lse, mask)
-        ctx.meta = (win, scale)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        q, k, v, out, lse, mask = ctx.saved_tensors
-        win, scale = ctx.meta
-        do = _rows16(do.to(q.dtype))
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        _backward(q, k, v, out, do, dq, dk, dv, mask, win, scale, lse)
-        return dq, dk, dv, None, None, None
 
 
 def visible(L: int, left: Optional[int], right: Optional[int], sinks: int, device=None) -> torch.Tensor:
@@ -187,12 +157,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
         raise ValueError(f"window_attention: length {L} is over {MAX_LEN}")
     if q.numel() == 0:
         return q * 1.0
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _WindowAttnFn.apply(q, k, v, mask, win, scale)
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    out = torch.empty(N, L, H, d, dtype=q.dtype, device=q.device)
-    _forward(q, k, v, out, mask, win, scale, None)
-    return out
+    return _native.binding().window_attention(q, k, v, mask, *win, scale)
 
 
 class _PackedWindowAttnFn(torch.autograd.Function):
