@@ -52,6 +52,7 @@ struct Args {
   int mask_bytes;
   float* lse;  // (N, H, L)  minus the log-sum-exp of a row's scores (log2 units, scale included); null: not kept
   float* dd;   // (N, H, L)  minus D
+  unsigned char* rest;  // rest_at: the next 8 bits of o below its bf16 (signed); with lse
   int L, H, G;  // G = query heads per key/value head
   int left, right, sinks;
   float scale;
@@ -61,6 +62,25 @@ struct Args {
   long far_main;  // slots of the near parts
   int far_chunks, far_blocks, far_tile;
 };
+
+// What rounding a float to bf16 hi left out, to 2^-8 of hi's last place: D = do.o is subtracted from do.v_j, and with
+// the rounded o the gradients of a narrow window were off by 0.0029 of their size (norms), with these bits by
+// 0.0025, of which 0.0024 is the rounding of dS and of the result.  One byte per element, 3 to 5 % of the time of forward
+// and backward (32 pages x 2000 tokens x 12 heads: 631 -> 650 us).
+__device__ __forceinline__ int rest_of(float x, unsigned hi) {
+  const int r = (int)(__builtin_bit_cast(unsigned, x) - (hi << 16));
+  return min(max((r + 128) >> 8, -128), 127);
+}
+// Laid out for the two kernels' lanes, (N, H, ceil(L / 32), d / 8, 32 rows, 8): each store and load of a wave covers
+// 256 bytes in a row (in o's own
+// order, 8 bytes to a row at a time, forward and backward of the same pages took 666 us).
+template <int D>
+__device__ __forceinline__ unsigned char* rest_at(const Args& a, int n, int hd, int i, int eighth) {
+  return a.rest + ((((long)n * a.H + hd) * ((a.L + 31) >> 5) + (i >> 5)) * (D / 8) + eighth) * 256 + (i & 31) * 8;
+}
+__device__ __forceinline__ float with_rest(unsigned short hi, int rest) {
+  return __builtin_bit_cast(float, ((unsigned)hi << 16) + (unsigned)(rest << 8));
+}
 
 #define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16((a), (b), (c), 0, 0, 0)
 
@@ -425,12 +445,21 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
   unsigned short* orow = a.o.p + n * a.o.n + (long)i * a.o.l + hd * a.o.h;
 #pragma unroll
+  for (int e = 0; e < D / 32; ++e) o[e] *= inv;
+#pragma unroll
   for (int e = 0; e < D / 32; ++e)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      *reinterpret_cast<uint2*>(orow + e * 32 + 8 * t + 4 * h) =
-          uint2{pack_bf16x2(o[e][4 * t] * inv, o[e][4 * t + 1] * inv),
-                pack_bf16x2(o[e][4 * t + 2] * inv, o[e][4 * t + 3] * inv)};
+    for (int t = 0; t < 4; ++t) {
+      const uint2 w{pack_bf16x2(o[e][4 * t], o[e][4 * t + 1]), pack_bf16x2(o[e][4 * t + 2], o[e][4 * t + 3])};
+      *reinterpret_cast<uint2*>(orow + e * 32 + 8 * t + 4 * h) = w;
+      if (a.lse) {
+        unsigned rest = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          rest |= (unsigned)(rest_of(o[e][4 * t + u], ((u < 2 ? w.x : w.y) >> (16 * (u & 1))) & 0xffffu) & 0xff) << (8 * u);
+        *reinterpret_cast<unsigned*>(rest_at<D>(a, n, hd, i, 4 * e + t) + 4 * h) = rest;
+      }
+    }
   if (a.lse && h == 0)
     a.lse[((long)n * a.H + hd) * a.L + i] = l == 0.f ? -INFINITY : -fmaf(m, sl, __log2f(l));
 }
@@ -456,10 +485,13 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
     bf16x8 of[D / 16];
     glob_frag<D>(a.o.p + n * a.o.n + (long)ic * a.o.l + hd * a.o.h, i < a.L, of);
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s)
+    for (int s = 0; s < D / 16; ++s) {
+      const uint2 rest = *reinterpret_cast<const uint2*>(rest_at<D>(a, n, hd, ic, 2 * s + h));
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        dd = fmaf(bf16_to_f32((unsigned short)of[s][e]), bf16_to_f32((unsigned short)gf[s][e]), dd);
+        dd = fmaf(with_rest((unsigned short)of[s][e], (int)((e < 4 ? rest.x : rest.y) << (24 - 8 * (e & 3))) >> 24),
+                  bf16_to_f32((unsigned short)gf[s][e]), dd);
+    }
   }
   dd += other_half(dd, h);
   const long row = ((long)n * a.H + hd) * a.L + ic;
@@ -819,7 +851,7 @@ using namespace pv::wattn;
 
 namespace {
 Args common(const void* q, const void* k, const void* v, const void* o, const long* st, const void* mask, long mask_n,
-            int mask_bytes, float* lse, int L, int H, int G, int left, int right, int sinks, float scale) {
+            int mask_bytes, float* lse, void* rest, int L, int H, int G, int left, int right, int sinks, float scale) {
   Args a{};
   a.q = view(q, st, 0);
   a.k = view(k, st, 1);
@@ -829,6 +861,7 @@ Args common(const void* q, const void* k, const void* v, const void* o, const lo
   a.mask_n = mask_n;
   a.mask_bytes = mask_bytes;
   a.lse = lse;
+  a.rest = static_cast<unsigned char*>(rest);
   a.L = L, a.H = H, a.G = G;
   a.left = min(left, L), a.right = min(right, L), a.sinks = min(sinks, L);
   a.scale = scale;
@@ -838,12 +871,14 @@ Args common(const void* q, const void* k, const void* v, const void* o, const lo
 }  // namespace
 
 // q, o (N, L, H, d), k, v (N, L, H / G, d) bf16; st: element strides {n, l, h} of q, k, v, o
-// (multiples of 8, 16-byte aligned pointers); left, right >= L: unbounded.  lse (N, H, L) fp32 or null.
+// (multiples of 8, 16-byte aligned pointers); left, right >= L: unbounded.  lse (N, H, L) fp32 and
+// rest (N * H * ceil(L / 32) * 32 * d bytes) for the backward pass, or both null.
 PV_API int pv_wattn_fwd(const void* q, const void* k, const void* v, void* o, const long* st, const void* mask,
-                        long mask_n, int mask_bytes, float* lse, int N, int L, int H, int G, int d, int left,
-                        int right, int sinks, float scale, void* stream) {
+                        long mask_n, int mask_bytes, float* lse, void* rest, int N, int L, int H, int G, int d,
+                        int left, int right, int sinks, float scale, void* stream) {
   if (const int rc = check_sizes(N, L, H, G, d, scale)) return rc;
-  const Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, L, H, G, left, right, sinks, scale);
+  if (!lse != !rest) return -5;
+  const Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, rest, L, H, G, left, right, sinks, scale);
   const dim3 grid((unsigned)((long)a.tiles * H * N));
   if (d == 32) hipLaunchKernelGGL(fwd_kernel<32>, grid, dim3(NTH), 0, (hipStream_t)stream, a);
   else if (d == 64) hipLaunchKernelGGL(fwd_kernel<64>, grid, dim3(NTH), 0, (hipStream_t)stream, a);
@@ -860,11 +895,12 @@ PV_API long pv_wattn_bwd_ws(int N, int L, int H, int G, int d, int left, int sin
 // st: strides of q, k, v, o, go, dq, dk, dv.  dd (N, H, L) and ws fp32 workspace; dq (N, L, H, d), dk, dv
 // (N, L, H / G, d) bf16, every element written.
 PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const void* go, void* dq, void* dk,
-                        void* dv, const long* st, const void* mask, long mask_n, int mask_bytes, float* lse, float* dd,
-                        float* ws, long ws_floats, int N, int L, int H, int G, int d, int left, int right, int sinks,
+                        void* dv, const long* st, const void* mask, long mask_n, int mask_bytes, float* lse,
+                        const void* rest, float* dd, float* ws, long ws_floats, int N, int L, int H, int G, int d, int left, int right, int sinks,
                         float scale, void* stream) {
   if (const int rc = check_sizes(N, L, H, G, d, scale)) return rc;
-  Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, L, H, G, left, right, sinks, scale);
+  Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, const_cast<void*>(rest), L, H, G, left, right, sinks,
+                  scale);
   a.go = view(go, st, 4);
   a.dq = view(dq, st, 5);
   a.dk = view(dk, st, 6);

@@ -135,9 +135,9 @@ SIGS = {
     "pv_sumsq": "p" "l" "p" "p",
     "pv_scale": "p" "lf" "p",
     # window_attention.hip
-    "pv_wattn_fwd": "ppppp" "pli" "p" "iiiii" "iii" "f" "p",
+    "pv_wattn_fwd": "ppppp" "pli" "pp" "iiiii" "iii" "f" "p",
     "pv_wattn_bwd_ws": "iiiii" "ii",
-    "pv_wattn_bwd": "ppppp" "pppp" "pli" "pp" "pl" "iiiii" "iii" "f" "p",
+    "pv_wattn_bwd": "ppppp" "pppp" "pli" "ppp" "pl" "iiiii" "iii" "f" "p",
     # token_embedding.hip
     "pv_temb_fwd": "pipipi" "lli" "f" "pp" "ppi" "p",
     "pv_temb_grad_ws": "lli",

@@ -81,15 +81,15 @@ def _mask_args(mask: Optional[torch.Tensor]):
 
 # the packed form's calls (views of one buffer); the plain form's are in csrc/binding/autograd.cpp
 
-def _forward(q, k, v, out, mask, win, scale: float, lse) -> None:
+def _forward(q, k, v, out, mask, win, scale: float, lse, rest) -> None:
     N, L, H, d = q.shape
     st = _strides(q, k, v, out)
     with on_device(q):
-        check(lib().pv_wattn_fwd(P(q), P(k), P(v), P(out), st, *_mask_args(mask), P(lse), N, L, H, H // k.shape[2], d,
-                                 *win, scale, stream(q.device)), "pv_wattn_fwd")
+        check(lib().pv_wattn_fwd(P(q), P(k), P(v), P(out), st, *_mask_args(mask), P(lse), P(rest), N, L, H,
+                                 H // k.shape[2], d, *win, scale, stream(q.device)), "pv_wattn_fwd")
 
 
-def _backward(q, k, v, out, do, dq, dk, dv, mask, win, scale: float, lse) -> None:
+def _backward(q, k, v, out, do, dq, dk, dv, mask, win, scale: float, lse, rest) -> None:
     N, L, H, d = q.shape
     G = H // k.shape[2]
     D = torch.empty_like(lse)
@@ -98,7 +98,7 @@ def _backward(q, k, v, out, do, dq, dk, dv, mask, win, scale: float, lse) -> Non
     st = _strides(q, k, v, out, do, dq, dk, dv)
     with on_device(q):
         check(lib().pv_wattn_bwd(P(q), P(k), P(v), P(out), P(do), P(dq), P(dk), P(dv), st, *_mask_args(mask), P(lse),
-                                 P(D), P(ws), n, N, L, H, G, d, *win, scale, stream(q.device)), "pv_wattn_bwd")
+                                 P(rest), P(D), P(ws), n, N, L, H, G, d, *win, scale, stream(q.device)), "pv_wattn_bwd")
 
 
 def visible(L: int, left: Optional[int], right: Optional[int], sinks: int, device=None) -> torch.Tensor:
@@ -166,17 +166,18 @@ class _PackedWindowAttnFn(torch.autograd.Function):
     projection, so there are no splits, copies or gradient concatenations."""
 
     @staticmethod
-    def forward(ctx, qkv, masks, shapes, heads, win, scale):
+    def forward(ctx, qkv, masks, shapes, heads, win, scale, train):
         qkv = qkv.contiguous()
         C = qkv.shape[1]
         d = C // (3 * heads)
         out = torch.empty(qkv.shape[0], heads * d, dtype=qkv.dtype, device=qkv.device)
-        lses = []
+        stats = []  # per group: log-sum-exp, and the bits of out below its bf16
         for (q, k, v, o), m, (N, L) in zip(_groups(qkv, out, shapes, heads, d), masks, shapes):
-            lse = torch.empty(N, heads, L, dtype=torch.float32, device=qkv.device)
-            _forward(q, k, v, o, m, _window(*win, L), scale, lse)
-            lses.append(lse)
-        ctx.save_for_backward(qkv, out, *masks, *lses)
+            kept = (torch.empty(N, heads, L, dtype=torch.float32, device=qkv.device),
+                    torch.empty(N, heads, (L + 31) // 32 * 32, d, dtype=torch.uint8, device=qkv.device)) if train else (None, None)
+            _forward(q, k, v, o, m, _window(*win, L), scale, *kept)
+            stats += kept
+        ctx.save_for_backward(qkv, out, *masks, *stats)
         ctx.meta = (shapes, heads, d, win, scale)
         return out
 
@@ -186,15 +187,16 @@ class _PackedWindowAttnFn(torch.autograd.Function):
         shapes, heads, d, win, scale = ctx.meta
         n = len(shapes)
         qkv, out = ctx.saved_tensors[:2]
-        masks, lses = ctx.saved_tensors[2:2 + n], ctx.saved_tensors[2 + n:]
+        masks, stats = ctx.saved_tensors[2:2 + n], ctx.saved_tensors[2 + n:]
         do = do.to(qkv.dtype).contiguous()
         if do.data_ptr() % 16:
             do = do.clone()
         dqkv = torch.empty_like(qkv)
-        for (q, k, v, o), (dq, dk, dv, g), m, lse, (N, L) in zip(_groups(qkv, out, shapes, heads, d),
-                                                                 _groups(dqkv, do, shapes, heads, d), masks, lses, shapes):
-            _backward(q, k, v, o, g, dq, dk, dv, m, _window(*win, L), scale, lse)
-        return dqkv, None, None, None, None, None
+        for (q, k, v, o), (dq, dk, dv, g), m, lse, rest, (N, L) in zip(_groups(qkv, out, shapes, heads, d),
+                                                                       _groups(dqkv, do, shapes, heads, d), masks, stats[::2], stats[1::2],
+                                                                       shapes):
+            _backward(q, k, v, o, g, dq, dk, dv, m, _window(*win, L), scale, lse, rest)
+        return dqkv, None, None, None, None, None, None
 
 
 def _groups(qkv, out, shapes, heads: int, d: int):
@@ -221,7 +223,8 @@ def packed_window_attention(qkv: torch.Tensor, masks: Sequence[Optional[torch.Te
     masks = [_key_mask(m, N, L, qkv.device) for m, (N, L) in zip(masks, shapes)]
     if use_hip(qkv) and qkv.dtype == torch.bfloat16 and d in HEAD_DIMS and min((n for s in shapes for n in s), default=0) > 0 \
             and qkv.data_ptr() % 16 == 0:
-        return _PackedWindowAttnFn.apply(qkv, masks, shapes, heads, (left, right, sinks), _scale(None, d))
+        return _PackedWindowAttnFn.apply(qkv, masks, shapes, heads, (left, right, sinks), _scale(None, d),
+                                         torch.is_grad_enabled() and qkv.requires_grad)
     outs, off = [], 0
     for (N, L), m in zip(shapes, masks):
         x = qkv[off:off + N * L].view(N, L, 3, heads, d)

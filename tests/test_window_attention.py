@@ -8,7 +8,7 @@ matrices.  One rounding to bf16 is off by at most h = 2^-8 relative.
   magnitudes, log2e and the subtraction of the maximum add a few 2^-24 of the same size; twice that,
   as a relative error of p, is e = 2^-23 (d + 16) max scale |q||k| + 2^-17 (the 2^-17 covers the
   hardware exponential, the logarithm and the row sum's up to 2^6 half steps);
-* D is taken with the rounded o: off by |do| (h P|V| + h |o|);
+* D is taken with o before its last rounding (here with it): off by |do| (h P|V| + h |o|) at most;
 * dS = p (dP - D) is rounded once: its error E = p (err D + d 2^-23 |do||v|) + (h + e) |dS|;
   dq, dk: E against |k|, |q| and one rounding; dv: (h + e) P^T|do| and one rounding.
 """
@@ -249,6 +249,31 @@ def test_far_queries_of_the_sinks(d, L, left, right, sinks):
         m = ragged(3, L, 2, holes=True)
         m[1, :7] = False                     # a masked sink
         check(*inputs(3, L, 2, 2, d, L + 1), left, right, sinks, m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("L", [3, 40, 131])
+def test_row_sums_of_the_gradient_are_exact_enough_for_values_far_from_zero(d, L):
+    """Values around 64: D and do.v_j are large and nearly cancel.  With q = 0 every probability is 1 / keys from
+    exponentials that are exactly 1, so D's error is o's alone: kept to 2^-8 of its last bf16 place (off by 2^-15 |o| at
+    most), not to bf16 (2^-8).  fp32: the products of d terms and the start value D are off by d 2^-23 of the sum of
+    magnitudes each; p and the quotient by 2^-17.  Then dS and dq are rounded once."""
+    _, k, v, do = inputs(2, L, 2, 2, d, 11, device="cpu")
+    v = (v.float() + 64).bfloat16()
+    q = torch.zeros_like(k)
+    res, _ = oracle(q, k, v, do, 1, 1, 0, None)
+    K, V, dO, O = (t.double().transpose(1, 2) for t in (k, v, do, res[0]))
+    see = visible(L, 1, 1, 0)
+    P = see.double() / see.double().sum(-1, keepdim=True)
+    dP = dO @ V.transpose(-1, -2)
+    dS = P * (dP - (dO * O).sum(-1, keepdim=True))
+    E = P * (2.0 ** -15 * (dO.abs() * O.abs()).sum(-1, keepdim=True) + 2 * d * 2.0 ** -23 * dO.abs() @ V.abs().transpose(-1, -2))
+    E = E + (H_ + 2.0 ** -17) * dS.abs()
+    tol = (E @ K.abs()).transpose(1, 2) / math.sqrt(d) + H_ * res[1].abs() + 1e-30
+    qg = q.cuda().requires_grad_()
+    window_attention(qg, k.cuda(), v.cuda(), 1, 1).backward(do.cuda())
+    close(qg.grad, res[1], tol, "dq")
 
 
 @pytest.mark.gpu
