@@ -10,15 +10,11 @@
 // ids (a word of a Zipf text is several percent of all tokens).  Here every row has one writer:
 //   * few tokens (T <= SMALL_T): one launch.  A workgroup per token; the first token of an id adds
 //     all rows of that id, found by comparing ids; other workgroups zero the rows without a token.
-//   * else the tokens are sorted by id (radix_sort.hip, stable), a wave adds the rows of CHUNK
+//   * else the tokens are sorted by id (two launches per 8 bits, which zero the gradient on the way; stable), a wave adds the rows of CHUNK
 //     consecutive sorted tokens, writing the runs that lie inside its chunk, and the runs that
 //     cross a chunk's border are joined from the chunks' fp32 partial rows by a second launch.
 // All sums are fp32, in an order that depends on the sizes and ids alone.
 #include "common.h"
-
-PV_API long pv_rsort_temp_bytes(long n, int end_bit, int key_bytes);
-PV_API int pv_rsort_pairs(void* temp, long temp_bytes, const void* keys_in, void* keys_out, const unsigned* vals_in,
-                          unsigned* vals_out, long n, int end_bit, int key_bytes, void* stream);
 
 namespace pv {
 namespace temb {
@@ -172,9 +168,9 @@ struct Cols {
 
 __device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Sum over the four waves of a workgroup in wave order, into wave 0's x
-template <typename X, int W>
-__device__ __forceinline__ void join_waves(X& x, float (&sh)[3][W][64]) {
+// Sum over the N + 1 waves of a workgroup in wave order, into wave 0's x
+template <typename X, int W, int N>
+__device__ __forceinline__ void join_waves(X& x, float (&sh)[N][W][64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (wave)
 #pragma unroll
@@ -184,7 +180,7 @@ __device__ __forceinline__ void join_waves(X& x, float (&sh)[3][W][64]) {
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int w = 0; w < 3; ++w) x.a[i] += sh[w][i][lane];
+      for (int w = 0; w < N; ++w) x.a[i] += sh[w][i][lane];
 }
 
 // Few tokens.  Workgroup b < T: token b, which writes its id's row if it is the id's first token
@@ -222,7 +218,7 @@ __global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __re
           if (i < n) sum.add(row[i]);
       }
     }
-    join_waves<Cols<TG, W>, W>(sum, sh);
+    join_waves<Cols<TG, W>, W, 3>(sum, sh);
     if (wave == 0) sum.store(dW + (size_t)v * E, E, scale, acc);
     return;
   }
@@ -248,16 +244,134 @@ __global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __re
   }
 }
 
-// Sort keys of the tokens; the same launch zeroes the gradient (z floats at dW)
+// ---- sort by id: 8 bits at a time, least significant first, stable
+// The tokens lie in at most PARTS parts of whole tiles, one per workgroup.  count_kernel: how many tokens of each
+// part have which digit.  place_kernel: every workgroup adds up that table for itself (a part's digit starts
+// behind the smaller digits of all parts and its own digit in the parts before; no launch for the sums) and moves its tokens.
+// Few workgroups and short ones, bound by latency; the zeroing of the gradient is spread over these launches as further
+// workgroups, whose writes run meanwhile.  At 73728 tokens, 30522 rows of 768: 30 us, where a launch that zeroes
+// and the general sort's six launches took 46.
+constexpr int TILE = 1024;   // threads of a workgroup, a token each
+constexpr int PARTS = 128;
+constexpr int ZFILL = 512;   // zeroing workgroups per launch, at most
+
 template <typename KT>
-__global__ __launch_bounds__(256) void key_kernel(Ids ids, KT* __restrict__ keys, long T, long V, long pad,
-                                                  float* __restrict__ dW, long z) {
-  const long i0 = (long)blockIdx.x * 256 + threadIdx.x, n = (long)gridDim.x * 256;
-  for (long t = i0; t < T; t += n) keys[t] = (KT)ids.key(t, V, pad);
-  const bool vec = (reinterpret_cast<size_t>(dW) & 15) == 0;
-  const long z4 = vec ? z / 4 : 0;
-  for (long i = i0; i < z4; i += n) reinterpret_cast<f32x4*>(dW)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (long i = z4 * 4 + i0; i < z; i += n) dW[i] = 0.f;
+struct Tokens {  // keys and token numbers; from the ids themselves if keys is null
+  Ids ids;
+  long V, pad;
+  const KT* keys;
+  const unsigned* slot;
+  __device__ __forceinline__ unsigned key(long t) const { return keys ? (unsigned)keys[t] : ids.key(t, V, pad); }
+};
+
+struct Fill {  // n floats at p, this launch's share of the gradient
+  float* p;
+  long n;
+  __device__ __forceinline__ void run(int wg, int wgs) const {
+    const long i0 = (long)wg * TILE + threadIdx.x, step = (long)wgs * TILE;
+    const long n4 = (reinterpret_cast<size_t>(p) & 15) == 0 ? n / 4 : 0;
+    for (long i = i0; i < n4; i += step) reinterpret_cast<f32x4*>(p)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (long i = n4 * 4 + i0; i < n; i += step) p[i] = 0.f;
+  }
+};
+
+// the wave's lanes that hold a token of the same digit as this one
+__device__ __forceinline__ unsigned long long same_digit(unsigned digit, bool here) {
+  unsigned long long m = __ballot(here);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const unsigned long long one = __ballot((digit >> b) & 1u);
+    m &= (digit >> b) & 1u ? one : ~one;
+  }
+  return m;
+}
+
+template <typename KT>
+__global__ __launch_bounds__(TILE) void count_kernel(Tokens<KT> src, long T, long part, int parts, int shift,
+                                                     unsigned* __restrict__ table, Fill fill) {
+  if ((int)blockIdx.x >= parts) return fill.run((int)blockIdx.x - parts, (int)gridDim.x - parts);
+  __shared__ unsigned n[256];
+  if (threadIdx.x < 256) n[threadIdx.x] = 0;
+  __syncthreads();
+  const long b = (long)blockIdx.x * part, e = min(T, b + part);
+  for (long t0 = b; t0 < e; t0 += TILE) {
+    const long t = t0 + threadIdx.x;
+    const bool here = t < e;
+    const unsigned digit = here ? (src.key(t) >> shift) & 255u : 0u;
+    const unsigned long long m = same_digit(digit, here);
+    if (here && (threadIdx.x & 63) == (unsigned)__builtin_ctzll(m)) atomicAdd(&n[digit], (unsigned)__popcll(m));
+  }
+  __syncthreads();
+  if (threadIdx.x < 256) table[(size_t)blockIdx.x * 256 + threadIdx.x] = n[threadIdx.x];
+}
+
+template <typename KT>
+__global__ __launch_bounds__(TILE) void place_kernel(Tokens<KT> src, long T, long part, int parts, int shift,
+                                                     const unsigned* __restrict__ table, KT* __restrict__ keys,
+                                                     unsigned* __restrict__ slot, Fill fill) {
+  if ((int)blockIdx.x >= parts) return fill.run((int)blockIdx.x - parts, (int)gridDim.x - parts);
+  __shared__ unsigned base[256], before[4][256], all[4][256], waves[4];
+  __shared__ unsigned short in[TILE / 64][256];  // tokens of the tile per wave and digit, then those of the waves before
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = threadIdx.x & 255, quarter = threadIdx.x >> 8;
+  {
+    unsigned x = 0, y = 0;
+#pragma unroll 8
+    for (int p = quarter; p < parts; p += 4) {
+      const unsigned n = table[(size_t)p * 256 + d];
+      y += n;
+      x += p < (int)blockIdx.x ? n : 0u;
+    }
+    before[quarter][d] = x;
+    all[quarter][d] = y;
+  }
+  __syncthreads();
+  unsigned sum = 0, own = 0;
+  if (quarter == 0) {  // running sum over the digits: within each of four waves, then over them
+    own = all[0][d] + all[1][d] + all[2][d] + all[3][d];
+    sum = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned v = __shfl_up(sum, o);
+      sum += lane >= o ? v : 0u;
+    }
+    if (lane == 63) waves[wave] = sum;
+  }
+  __syncthreads();
+  if (quarter == 0) {
+    sum -= own;
+    for (int w = 0; w < wave; ++w) sum += waves[w];
+    base[d] = sum + before[0][d] + before[1][d] + before[2][d] + before[3][d];
+  }
+  const long b = (long)blockIdx.x * part, e = min(T, b + part);
+  for (long t0 = b; t0 < e; t0 += TILE) {
+    const long t = t0 + threadIdx.x;
+    const bool here = t < e;
+    const unsigned key = here ? src.key(t) : 0u, tok = here ? (src.keys ? src.slot[t] : (unsigned)t) : 0u;
+    const unsigned digit = (key >> shift) & 255u;
+#pragma unroll
+    for (int u = 0; u < TILE / 64 / 4; ++u) in[4 * u + quarter][d] = 0;
+    __syncthreads();
+    const unsigned long long m = same_digit(digit, here);
+    const int rank = __popcll(m & ((1ull << lane) - 1ull));
+    if (here && rank == 0) in[wave][digit] = (unsigned short)__popcll(m);
+    __syncthreads();
+    unsigned n = 0;
+    if (quarter == 0)
+#pragma unroll
+      for (int w = 0; w < TILE / 64; ++w) {
+        const unsigned x = in[w][d];
+        in[w][d] = (unsigned short)n;
+        n += x;
+      }
+    __syncthreads();
+    if (here) {
+      const unsigned to = base[digit] + in[wave][digit] + (unsigned)rank;
+      keys[to] = (KT)key;
+      slot[to] = tok;
+    }
+    __syncthreads();
+    if (quarter == 0) base[d] += n;
+  }
 }
 
 // A wave adds the rows of its chunk of the sorted tokens, run by run.  Partial rows: slot 2 c = the
@@ -316,14 +430,16 @@ __global__ __launch_bounds__(256) void walk_kernel(const KT* __restrict__ keys, 
 }
 
 // Where a run begins in chunk c and goes on behind it: the sum of its partial rows.  A wave per chunk; runs over
-// many chunks (frequent ids) are added by the workgroup's four waves together, a quarter each.
+// many chunks (frequent ids) are added by the workgroup's four waves together, a quarter each (sixteen waves: 30 us
+// instead of 20 at 256000 tokens x 512).
 constexpr int ALONE = 16;  // partial rows that a wave adds by itself
+constexpr int JOIN = 4;   // waves per workgroup
 template <typename TG, typename KT, int W>
-__global__ __launch_bounds__(256) void join_kernel(const KT* __restrict__ keys, const float* __restrict__ part,
+__global__ __launch_bounds__(64 * JOIN) void join_kernel(const KT* __restrict__ keys, const float* __restrict__ part,
                                                    float* __restrict__ dW, long T, long V, int E, float scale,
                                                    int acc) {
-  __shared__ float sh[3][W][64];
-  __shared__ long many[4];
+  __shared__ float sh[JOIN - 1][W][64];
+  __shared__ long many[JOIN];
   const int wave = threadIdx.x >> 6;
   auto total = [&](long c, long x0, long x1) {  // partial rows x0 .. of the run that begins in chunk c
     Cols<float, W> sum, row;
@@ -336,7 +452,7 @@ __global__ __launch_bounds__(256) void join_kernel(const KT* __restrict__ keys, 
     return sum;
   };
   {
-    const long c = (long)blockIdx.x * 4 + wave, b = c * CHUNK, e = b + CHUNK;
+    const long c = (long)blockIdx.x * JOIN + wave, b = c * CHUNK, e = b + CHUNK;
     long m = 0;
     if (e < T) {
       const KT key = keys[e - 1];
@@ -354,12 +470,12 @@ __global__ __launch_bounds__(256) void join_kernel(const KT* __restrict__ keys, 
     if ((threadIdx.x & 63) == 0) many[wave] = m > ALONE ? m : 0;
   }
   __syncthreads();
-  for (int w = 0; w < 4; ++w) {
-    const long m = many[w], c = (long)blockIdx.x * 4 + w;
+  for (int w = 0; w < JOIN; ++w) {
+    const long m = many[w], c = (long)blockIdx.x * JOIN + w;
     if (!m) continue;
-    const long q = (m + 3) / 4, x0 = wave * q;
+    const long q = (m + JOIN - 1) / JOIN, x0 = wave * q;
     Cols<float, W> sum = total(c, x0, min(m, x0 + q));
-    join_waves<Cols<float, W>, W>(sum, sh);
+    join_waves<Cols<float, W>, W, JOIN - 1>(sum, sh);
     if (wave == 0) sum.store(dW + (size_t)keys[c * CHUNK + CHUNK - 1] * E, E, scale, acc);
     __syncthreads();
   }
@@ -368,48 +484,64 @@ __global__ __launch_bounds__(256) void join_kernel(const KT* __restrict__ keys, 
 __host__ inline size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct Layout {
-  size_t keys, skeys, slot, part, temp, bytes;
-  long temp_bytes, chunks;
-  int kb, bits;
+  size_t keys[2], slot[2], part, table, bytes;
+  long chunks, per;  // tokens per part of the sort
+  int kb, passes, parts;
 };
 
 __host__ inline Layout layout(long T, long V, int E) {
   Layout l{};
   if (T <= SMALL_T) return l;
   l.kb = V < 65536 ? 2 : 4;
-  while ((1L << l.bits) <= V) ++l.bits;  // keys 0 .. V
+  l.passes = 1;
+  while ((1L << (8 * l.passes)) <= V) ++l.passes;  // keys 0 .. V
   l.chunks = (T + CHUNK - 1) / CHUNK;
+  l.per = ((T + PARTS - 1) / PARTS + TILE - 1) / TILE * TILE;
+  l.parts = (int)((T + l.per - 1) / l.per);
   size_t o = 0;
-  l.keys = o;
-  o = up(o + (size_t)T * l.kb);
-  l.skeys = o;
-  o = up(o + (size_t)T * l.kb);
-  l.slot = o;
-  o = up(o + (size_t)T * 4);
+  for (int i = 0; i < (l.passes > 1 ? 2 : 1); ++i) {
+    l.keys[i] = o;
+    o = up(o + (size_t)T * l.kb);
+    l.slot[i] = o;
+    o = up(o + (size_t)T * 4);
+  }
   l.part = o;
   o = up(o + (size_t)l.chunks * 2 * E * 4);
-  l.temp = o;
-  l.temp_bytes = pv_rsort_temp_bytes(T, l.bits, l.kb);
-  l.bytes = up(o + (size_t)l.temp_bytes);
+  l.table = o;
+  l.bytes = up(o + (size_t)l.parts * 256 * 4);
   return l;
 }
 
 template <typename TG, typename KT, int W>
 int sorted_grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc,
                 char* ws, const Layout& l, hipStream_t st) {
-  KT *keys = (KT*)(ws + l.keys), *sk = (KT*)(ws + l.skeys);
-  unsigned* slot = (unsigned*)(ws + l.slot);
   float* part = (float*)(ws + l.part);
-  const long z = acc ? 0 : V * E;
-  const long want = (max(T, z / 4) + 255) / 256;
-  hipLaunchKernelGGL((key_kernel<KT>), dim3((unsigned)min(want, 4096L)), dim3(256), 0, st, ids, keys, T, V, pad, dW, z);
-  PV_LAUNCH_CHECK();
-  if (const int rc = pv_rsort_pairs(ws + l.temp, l.temp_bytes, keys, sk, nullptr, slot, T, l.bits, l.kb, st)) return rc;
+  unsigned* table = (unsigned*)(ws + l.table);
+  const long z = acc ? 0 : V * E, share = (z / (2 * l.passes) + 3) & ~3L;
+  Tokens<KT> src{ids, V, pad, nullptr, nullptr};
+  for (int k = 0; k < 2 * l.passes; ++k) {
+    const long z0 = min(z, k * share), z1 = k + 1 == 2 * l.passes ? z : min(z, z0 + share);
+    const Fill fill{dW + z0, z1 - z0};
+    const dim3 grid((unsigned)(l.parts + min((fill.n + 4 * TILE - 1) / (4 * TILE), (long)ZFILL)));
+    KT* keys = (KT*)(ws + l.keys[k / 2 & 1]);
+    unsigned* slot = (unsigned*)(ws + l.slot[k / 2 & 1]);
+    if (k % 2 == 0) {
+      hipLaunchKernelGGL((count_kernel<KT>), grid, dim3(TILE), 0, st, src, T, l.per, l.parts, 4 * k, table, fill);
+    } else {
+      hipLaunchKernelGGL((place_kernel<KT>), grid, dim3(TILE), 0, st, src, T, l.per, l.parts, 4 * (k - 1),
+                         (const unsigned*)table, keys, slot, fill);
+      src.keys = keys;
+      src.slot = slot;
+    }
+    PV_LAUNCH_CHECK();
+  }
+  const KT* sk = src.keys;
+  const unsigned* slot = src.slot;
   const int slabs = (E + 64 * W - 1) / (64 * W);
   hipLaunchKernelGGL((walk_kernel<TG, KT, W>), dim3((unsigned)((l.chunks + 3) / 4), slabs), dim3(256), 0, st,
-                     (const KT*)sk, (const unsigned*)slot, g, part, dW, T, V, E, scale, acc);
+                     sk, slot, g, part, dW, T, V, E, scale, acc);
   PV_LAUNCH_CHECK();
-  hipLaunchKernelGGL((join_kernel<TG, KT, W>), dim3((unsigned)((l.chunks + 3) / 4), slabs), dim3(256), 0, st, (const KT*)sk,
+  hipLaunchKernelGGL((join_kernel<TG, KT, W>), dim3((unsigned)((l.chunks + JOIN - 1) / JOIN), slabs), dim3(64 * JOIN), 0, st, sk,
                      (const float*)part, dW, T, V, E, scale, acc);
   PV_LAUNCH_CHECK();
   return 0;

@@ -99,6 +99,13 @@ def test_tables(V, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,E", [(131072, 200, 8), (131073, 3000, 4), (300001, 70000, 3), (2100, 1 << 24, 1)])
+def test_sort_of_many_tokens(T, V, E):
+    """Parts of several tiles with a ragged last one; one to four passes over the ids' bits."""
+    check(zipf(T, V, 5), V, E, torch.float32, 7)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("E", [1021, 1024, 1028, 2500])
 @pytest.mark.parametrize("T", [100, 4000])
 def test_wide_rows(E, T):
