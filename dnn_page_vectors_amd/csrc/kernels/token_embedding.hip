@@ -19,6 +19,9 @@
 namespace pv {
 namespace temb {
 
+// Up to here one launch, which compares every token with all others: at 2048 tokens 10 / 12 / 27 / 28 us where sorting
+// takes 31 / 30 / 42 / 48 (tables of 5000 x 64, 1024 x 300, 30522 x 768, 60000 x 512, Zipf ids).  Ids that are spread like this
+// meet between 3000 and 8000 tokens, but 2048 tokens of a single id are 87 against 28 us, and twice as many 173.
 constexpr int SMALL_T = 2048;
 constexpr int CHUNK = 32;  // sorted tokens per wave
 constexpr int ZROWS = 64;  // table rows per zeroing workgroup of the small path

@@ -60,7 +60,7 @@ struct Args {
   // backward: the sinks' far queries (see bwd_dkv_kernel); far_chunks = 0: not split off
   float* part;
   long far_main;  // slots of the near parts
-  int far_chunks, far_blocks, far_tile;
+  int far_chunks, far_blocks, far_tile, far_wgs;  // far_wgs: workgroups per sequence and key/value head
 };
 
 // What rounding a float to bf16 hi left out, to 2^-8 of hi's last place: D = do.o is subtracted from do.v_j, and with
@@ -549,7 +549,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
 //
 // The sinks are seen by every later query: walked by their own workgroup alone they would make it the last
 // by far.  Their far queries (behind the window's tiles) are dealt to workgroups of FAR tiles each, whose
-// waves share 32 keys and split the queries; partial sums in fp32, added up by sink_sum_kernel.
+// waves share 32 keys and split the queries; partial sums in fp32, added up by sink_sum_kernel.  They
+// are further workgroups of their head in the same launch, whose reads of Q and dO the others bring to the XCD's L2
+// (a launch of their own: 47 + 174 us against 189 at 64 pages x 975 tokens x 12 heads, 4 sinks; in the dq kernel, which
+// has the queries at hand, they cost as much as on their own).
 template <int D>
 struct KeyGrads {
   bf16x8 kf[D / 16], vf[D / 16];
@@ -626,79 +629,18 @@ __device__ __forceinline__ bool key_lane(const Args& a, int n, int kvh, int j, K
 }
 
 template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 2 : 1) void bwd_far_kernel(Args a) {
+__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short tiles[4][TK * D];  // Q, Q, dO, dO
   __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
-  const int lane = threadIdx.x & 63, wv = wave_id();
-  // ((sequence, head), chunk of query tiles), 32-key block of sinks
-  const int kb = blockIdx.x % a.far_blocks, slot = blockIdx.x / a.far_blocks;
-  const int ch = slot % a.far_chunks, nh = slot / a.far_chunks;
-  const int hd = nh % a.H, n = nh / a.H, w0 = kb * 32, j = w0 + (lane & 31);
-  const float sl = a.scale * LOG2E;
-  KeyGrads<D> w;
-  const bool ok = key_lane<D>(a, n, hd / a.G, j, w);
-  const unsigned long long okw = __ballot(ok);
-  Frags<D> fr;
-  fr.init();
-  Loader<D> lq, lg;
-  lq.init(a.q.p + n * a.q.n + (long)hd * a.q.h, a.q.l, tiles[0]);
-  lg.init(a.go.p + n * a.go.n + (long)hd * a.go.h, a.go.l, tiles[2]);
-  const float *rl = a.lse + ((long)n * a.H + hd) * a.L, *rd = a.dd + ((long)n * a.H + hd) * a.L;
-  const unsigned ls_at = lds_at(ls[0]), ds_at = lds_at(ds[0]);
-  const int t0 = a.far_tile + ch * FAR, t1 = min(t0 + FAR, (a.L + TK - 1) / TK);
-  if (okw != 0ull)
-    for (int t = t0; t < t1; t += 2) {  // two tiles at a time, one 32-row block per wave
-      const int n2 = min(2, t1 - t);
-      for (int u = 0; u < n2; ++u) {
-        lq.issue((t + u) * TK, a.L, u);
-        lg.issue((t + u) * TK, a.L, u);
-        if (wv == 0) floats_to_lds(rl, (t + u) * TK, a.L, ls_at + u * TK * 4);
-        if (wv == 1) floats_to_lds(rd, (t + u) * TK, a.L, ds_at + u * TK * 4);
-      }
-      landed();
-      __syncthreads();
-      const int u = wv >> 1, r0 = 32 * (wv & 1), i0 = (t + u) * TK + r0;
-      if (u < n2 && i0 < a.L) {
-        const unsigned see = ok && j < a.sinks ? bits_between(0, a.L - 1 - i0) : 0u;
-        w.block(fr, tiles[u], tiles[2 + u], r0, &ls[u][r0], &ds[u][r0], sl, see,
-                okw == ~0ull && w0 + 32 <= a.sinks && i0 + 32 <= a.L);
-      }
-      __syncthreads();
-    }
-  // the four waves' sums, added in wave order; wave wv finishes accumulator quad wv
-  float* red = reinterpret_cast<float*>(&tiles[0][0]);  // 4 x 1024 floats
-  static_assert(sizeof(tiles) >= 4 * 1024 * sizeof(float), "the waves' sums fit the tiles' place");
-  auto finish = [&](const f32x16& x, int which, int e) {
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 16; ++r) red[wv * 1024 + r * 64 + lane] = x[r];
-    __syncthreads();
-    f32x4 y;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      y[q] = red[(4 * wv + q) * 64 + lane];
-#pragma unroll
-      for (int v = 1; v < 4; ++v) y[q] += red[v * 1024 + (4 * wv + q) * 64 + lane];
-    }
-    if (j < a.sinks) *reinterpret_cast<f32x4*>(part_at<D>(a, a.far_main + slot, which, j, e, wv)) = y;
-  };
-#pragma unroll
-  for (int e = 0; e < D / 32; ++e) {
-    finish(w.dk[e], 0, e);
-    finish(w.dv[e], 1, e);
-  }
-}
-
-template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) unsigned short qt[2][TK * D];
-  __shared__ __attribute__((aligned(1024))) unsigned short gt[2][TK * D];
-  __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
+  unsigned short(*const qt)[TK * D] = tiles, (*const gt)[TK * D] = tiles + 2;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int Hkv = a.H / a.G;
-  const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
+  const Where wg(blockIdx.x, gridDim.x / (a.tiles + a.far_wgs), a.tiles + a.far_wgs);
   const int kvh = wg.nh % Hkv, n = wg.nh / Hkv;
-  const int b0 = wg.tile * RB, w0 = b0 + wave_id() * 32, j = w0 + (lane & 31);
+  // far: (head of the group, chunk of query tiles, 32-key block of sinks)
+  const bool far = wg.tile >= a.tiles;
+  const int x = wg.tile - a.tiles, gc = far ? x / a.far_blocks : 0, g0 = far ? gc / a.far_chunks : 0;
+  const int b0 = far ? 0 : wg.tile * RB, w0 = far ? x % a.far_blocks * 32 : b0 + wave_id() * 32, j = w0 + (lane & 31);
   const float sl = a.scale * LOG2E;
   const bool split = a.far_chunks != 0;
   KeyGrads<D> w;
@@ -707,9 +649,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   const bool all_ok = okw == ~0ull, any_ok = okw != 0ull;
   // queries that see a key of this workgroup: from b0 - right to the last key + left, or (sinks
   // that are not split off) to the end
-  const int lo = max(0, b0 - a.right) / TK;
-  const int last = b0 < a.sinks && !split ? a.L - 1 : min(a.L - 1, min(b0 + RB, a.L) - 1 + a.left);
-  const int per = last / TK - lo + 1, total = __syncthreads_or(any_ok) ? per * a.G : 0;
+  const int lo = far ? a.far_tile + gc % a.far_chunks * FAR : max(0, b0 - a.right) / TK;
+  const int last = far ? min(a.L, (lo + FAR) * TK) - 1
+                       : b0 < a.sinks && !split ? a.L - 1 : min(a.L - 1, min(b0 + RB, a.L) - 1 + a.left);
+  const int per = last / TK - lo + 1, total = __syncthreads_or(any_ok) ? (far ? per : per * a.G) : 0;
   // the same three kinds as in the forward, seen from the wave's keys
   const int none_lo = w0 - a.right - 31, none_hi = !any_ok ? -1 : w0 < a.sinks ? a.L - 1 : min(a.L - 1, w0 + 31 + a.left);
   const int full_lo = w0 + 31 - a.right;
@@ -718,9 +661,9 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   Frags<D> fr;
   fr.init();
   Loader<D> lq, lg;
-  lq.init(a.q.p + n * a.q.n + (long)kvh * a.G * a.q.h, a.q.l, qt[0]);
-  lg.init(a.go.p + n * a.go.n + (long)kvh * a.G * a.go.h, a.go.l, gt[0]);
-  const float *rl = a.lse + ((long)n * a.H + kvh * a.G) * a.L, *rd = a.dd + ((long)n * a.H + kvh * a.G) * a.L;
+  lq.init(a.q.p + n * a.q.n + (long)(kvh * a.G + g0) * a.q.h, a.q.l, qt[0]);
+  lg.init(a.go.p + n * a.go.n + (long)(kvh * a.G + g0) * a.go.h, a.go.l, gt[0]);
+  const float *rl = a.lse + ((long)n * a.H + kvh * a.G + g0) * a.L, *rd = a.dd + ((long)n * a.H + kvh * a.G + g0) * a.L;
   const unsigned ls_at = lds_at(ls[0]), ds_at = lds_at(ds[0]);
   int t1 = 0;  // the tile being read, within its head
   int buf = 1, i0t = 0;
@@ -738,7 +681,7 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int i0 = i0t + 32 * c;
-        if (i0 < none_lo || i0 > none_hi) continue;
+        if (i0 < none_lo || i0 > none_hi || (far && 2 * (it & 1) + c != wave_id())) continue;
         const bool full = i0 >= full_lo && i0 <= full_hi;
         unsigned see = 0u;
         if (!full) see = ok ? bits_between(j - a.right - i0, my_last - i0) : 0u;
@@ -758,6 +701,32 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
         rd += a.L;
       }
     }
+  }
+  if (far) {  // the four waves' sums, added in wave order; wave wv finishes accumulator quad wv
+    const int wv = wave_id();
+    const long slot = a.far_main + ((long)n * a.H + kvh * a.G + g0) * a.far_chunks + gc % a.far_chunks;
+    float* red = reinterpret_cast<float*>(&tiles[0][0]);  // 4 x 1024 floats
+    static_assert(sizeof(tiles) >= 4 * 1024 * sizeof(float), "the waves' sums fit the tiles' place");
+    auto finish = [&](const f32x16& x, int which, int e) {
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) red[wv * 1024 + r * 64 + lane] = x[r];
+      __syncthreads();
+      f32x4 y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        y[q] = red[(4 * wv + q) * 64 + lane];
+#pragma unroll
+        for (int v = 1; v < 4; ++v) y[q] += red[v * 1024 + (4 * wv + q) * 64 + lane];
+      }
+      if (j < a.sinks) *reinterpret_cast<f32x4*>(part_at<D>(a, slot, which, j, e, wv)) = y;
+    };
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      finish(w.dk[e], 0, e);
+      finish(w.dv[e], 1, e);
+    }
+    return;
   }
   if (split && j < a.sinks) {  // the sinks' near part: added to the far ones
 #pragma unroll
@@ -835,8 +804,8 @@ __host__ inline FarPlan far_plan(long N, long L, long H, long G, int d, int left
   f.tile = (int)first;
   f.chunks = (int)((tiles - first + FAR - 1) / FAR);
   f.blocks = (sinks + 31) / 32;
-  const long wgs = N * H * f.blocks * f.chunks;
-  if (wgs > (1L << 30)) return FarPlan{};
+  const long wgs = G * f.blocks * f.chunks;
+  if ((wgs + (L + RB - 1) / RB) * (H / G) * N > 0x7FFFFFFFL) return FarPlan{};
   f.wgs = (int)wgs;
   f.near_slots = N * (H / G);
   f.floats = (f.near_slots + N * H * f.chunks) * 2 * d * sinks;
@@ -913,13 +882,13 @@ PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void*
   a.far_blocks = f.blocks;
   a.far_tile = f.tile;
   a.far_main = f.near_slots;
-  const dim3 gq((unsigned)((long)a.tiles * H * N)), gk((unsigned)((long)a.tiles * (H / G) * N));
+  a.far_wgs = f.wgs;
+  const dim3 gq((unsigned)((long)a.tiles * H * N)), gk((unsigned)((long)(a.tiles + f.wgs) * (H / G) * N));
   hipStream_t s = (hipStream_t)stream;
 #define PV_WBWD(DV)                                                 \
   do {                                                              \
     hipLaunchKernelGGL(bwd_dq_kernel<DV>, gq, dim3(NTH), 0, s, a);  \
     PV_LAUNCH_CHECK();                                              \
-    if (f.wgs) hipLaunchKernelGGL(bwd_far_kernel<DV>, dim3(f.wgs), dim3(NTH), 0, s, a); \
     hipLaunchKernelGGL(bwd_dkv_kernel<DV>, gk, dim3(NTH), 0, s, a); \
     PV_LAUNCH_CHECK();                                              \
   } while (0)
