@@ -7,6 +7,7 @@
 // launchers' addresses are handed in by init(), so that the release and the debug library both work.
 // Arguments are checked in Python (ops/*.py) before they come here.
 #include <ATen/ATen.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -79,6 +80,21 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->requires_grad()) return true;
   return false;
+}
+
+// Autograd keeps one accumulation node per leaf, on the stream of the graph that first used it, for as long as a graph
+// holds it.  A captured backward would have to wait for that stream, which the capture does not survive (nor does
+// the process, when the broken graph is destroyed): such a capture is refused while it is still whole.
+void check_capture(std::initializer_list<const Tensor*> ts, const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : ts) {
+    if (!t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto s = node->stream();
+    TORCH_CHECK(s && *s == c10::hip::getCurrentHIPStream(t->get_device()).unwrap(), what,
+                ": a graph made on another stream still holds an argument of this capture (delete its outputs first)");
+  }
 }
 
 // ---- windowed attention ------------------------------------------------------------------------------------------
@@ -156,7 +172,10 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
 
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask, int64_t left,
                         int64_t right, int64_t sinks, double scale) {
-  if (wants_grad({&q, &k, &v})) return WindowAttention::apply(q, k, v, mask, left, right, sinks, scale);
+  if (wants_grad({&q, &k, &v})) {
+    check_capture({&q, &k, &v}, "window_attention");
+    return WindowAttention::apply(q, k, v, mask, left, right, sinks, scale);
+  }
   const c10::DeviceGuard guard(q.device());
   at::AutoDispatchBelowADInplaceOrView below;
   const Tensor qq = rows16(q), kk = rows16(k), vv = rows16(v);
@@ -210,7 +229,10 @@ struct ScaledEmbedding : torch::autograd::Function<ScaledEmbedding> {
 };
 
 Tensor scaled_embedding(const Tensor& W, const Tensor& ids, double scale, int64_t pad, bool bf16) {
-  if (wants_grad({&W})) return ScaledEmbedding::apply(W, ids, scale, pad, bf16);
+  if (wants_grad({&W})) {
+    check_capture({&W}, "scaled_embedding");
+    return ScaledEmbedding::apply(W, ids, scale, pad, bf16);
+  }
   const c10::DeviceGuard guard(W.device());
   at::AutoDispatchBelowADInplaceOrView below;
   return lookup(W.contiguous(), ids, scale, bf16);
@@ -286,6 +308,9 @@ PYBIND11_MODULE(pagevec_torch, m) {
   m.def("scaled_embedding", &scaled_embedding, call_guard<gil_scoped_release>());
   m.def("pack", &pack, call_guard<gil_scoped_release>());
   m.def("unpack", &unpack, call_guard<gil_scoped_release>());
-  m.def("bias_gelu8", [](const Tensor& x, const Tensor& b) { return Tensor(BiasGelu8::apply(x, b)); },
-        call_guard<gil_scoped_release>());
+  m.def("bias_gelu8", [](const Tensor& x, const Tensor& b) {
+    check_capture({&x, &b}, "ckpt8.bias_gelu");
+    return Tensor(BiasGelu8::apply(x, b));
+  }, call_guard<gil_scoped_release>());
+  m.def("check_capture", [](const Tensor& t, const char* what) { check_capture({&t}, what); });
 }

@@ -98,7 +98,9 @@ def unpack(p: Packed, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     dtype = p.dtype if dtype is None else dtype
     if dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"ckpt8.unpack: dtype must be bfloat16 or float32, got {dtype}")
-    D = p.q.shape[-1]
+    D = p.q.shape[-1] if p.q.dim() else 0
+    if D == 0:
+        raise ValueError(f"ckpt8.unpack: needs at least one column, got shape {tuple(p.q.shape)}")
     if p.q.dtype != torch.uint8 or p.s.dtype != torch.uint8 or p.s.shape != (*p.q.shape[:-1], _blocks(D)):
         raise ValueError(f"ckpt8.unpack: {tuple(p.q.shape)} {p.q.dtype} values do not go with {tuple(p.s.shape)} {p.s.dtype} scales")
     if p.q.device != p.s.device:

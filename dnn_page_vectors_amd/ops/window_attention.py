@@ -223,8 +223,10 @@ def packed_window_attention(qkv: torch.Tensor, masks: Sequence[Optional[torch.Te
     masks = [_key_mask(m, N, L, qkv.device) for m, (N, L) in zip(masks, shapes)]
     if use_hip(qkv) and qkv.dtype == torch.bfloat16 and d in HEAD_DIMS and min((n for s in shapes for n in s), default=0) > 0 \
             and qkv.data_ptr() % 16 == 0:
-        return _PackedWindowAttnFn.apply(qkv, masks, shapes, heads, (left, right, sinks), _scale(None, d),
-                                         torch.is_grad_enabled() and qkv.requires_grad)
+        train = torch.is_grad_enabled() and qkv.requires_grad
+        if train:
+            _native.binding().check_capture(qkv, "packed_window_attention")
+        return _PackedWindowAttnFn.apply(qkv, masks, shapes, heads, (left, right, sinks), _scale(None, d), train)
     outs, off = [], 0
     for (N, L), m in zip(shapes, masks):
         x = qkv[off:off + N * L].view(N, L, 3, heads, d)

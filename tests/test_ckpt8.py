@@ -5,6 +5,7 @@ independent fp64 computation.  GELU: the result is one bf16 rounding (2^-8) of a
 is off by a few 2^-24 times the exponent's argument a; |a| sg (1 - sg) stays below 1 where the factor
 q = 2k u + 6kc u^3 is below 64, so a slope is off by at most 2^-17 and y by 2^-20 |u|.
 """
+import gc
 import math
 
 import pytest
@@ -335,3 +336,50 @@ def test_gpu_refusals():
         ckpt8.bias_gelu(x.bfloat16(), torch.zeros(4))
     with pytest.raises(TypeError):
         ckpt8.pack(x.half())
+
+
+def test_unpack_refuses_no_columns():
+    empty = torch.zeros(3, 0, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        ckpt8.unpack(ckpt8.Packed(empty, empty, torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_capture_is_refused_while_an_eager_graph_holds_the_leaves():
+    """The refusal leaves the process and the stream usable; once the eager graph is gone the capture works."""
+    x = torch.randn(40, 96, device="cuda").bfloat16().requires_grad_()
+    b = torch.randn(96, device="cuda", requires_grad=True)
+    dy = torch.randn(40, 96, device="cuda").bfloat16()
+    y = ckpt8.bias_gelu(x, b)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ckpt8.bias_gelu(x, b)
+    want = torch.autograd.grad(y, (x, b), dy)
+    del y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ckpt8.bias_gelu(x, b), (x, b), dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_nothing_outlives_its_graph():
+    x = torch.randn(64, 128, device="cuda").bfloat16().requires_grad_()
+    b = torch.randn(128, device="cuda", requires_grad=True)
+    dy = torch.randn(64, 128, device="cuda").bfloat16()
+    gc.collect()
+    gc.disable()
+    try:
+        used = []
+        for _ in range(4):
+            torch.autograd.grad(ckpt8.bias_gelu(x, b), (x, b), dy)
+            ckpt8.bias_gelu(x, b)  # a graph without a backward
+            used.append(torch.cuda.memory_allocated())
+    finally:
+        gc.enable()
+    assert used[1] == used[-1]

@@ -228,6 +228,27 @@ def test_graph_replays_and_side_stream(T):
 
 
 @pytest.mark.gpu
+def test_capture_is_refused_while_an_eager_graph_holds_the_table():
+    W = torch.randn(50, 16, device="cuda", requires_grad=True)
+    ids = torch.arange(30, device="cuda")
+    g = torch.randn(30, 16, device="cuda")
+    out = scaled_embedding(ids, W, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            scaled_embedding(ids, W, out_dtype=torch.float32)
+    (want,) = torch.autograd.grad(out, W, g)
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(scaled_embedding(ids, W, out_dtype=torch.float32), W, g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_gpu_refusals():
     ids = torch.tensor([0], device="cuda")
     with pytest.raises(TypeError):

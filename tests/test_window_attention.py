@@ -12,6 +12,7 @@ matrices.  One rounding to bf16 is off by at most h = 2^-8 relative.
 * dS = p (dP - D) is rounded once: its error E = p (err D + d 2^-23 |do||v|) + (h + e) |dS|;
   dq, dk: E against |k|, |q| and one rounding; dv: (h + e) P^T|do| and one rounding.
 """
+import gc
 import math
 
 import pytest
@@ -411,6 +412,53 @@ def test_gradient_against_differences():
         curve = abs((exact[0] - exact[1]) / (2 * eps) - want)
         slack = room / (2 * eps) + curve + float((gt[n] * dirs[n].double().cpu().abs()).sum())
         assert abs((vals[0] - vals[1]) / (2 * eps) - inner) <= slack
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_capture_is_refused_while_an_eager_graph_holds_the_operands(packed):
+    x = torch.randn(2 * 40, 3 * 2 * 32, device="cuda").bfloat16().requires_grad_()
+    do = torch.randn(2 * 40, 2 * 32, device="cuda").bfloat16()
+
+    def call():
+        if packed:
+            return packed_window_attention(x, [None], [(2, 40)], 2, 8, 8)
+        y = x.detach().view(2, 40, 3, 2, 32)
+        return window_attention(q, y[:, :, 1], y[:, :, 2], 8, 8).reshape(80, 64)
+
+    q = x.detach().view(2, 40, 3, 2, 32)[:, :, 0].contiguous().requires_grad_()
+    leaf = x if packed else q
+    out = call()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()
+    (want,) = torch.autograd.grad(out, leaf, do)
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(call(), leaf, do)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_nothing_outlives_its_graph():
+    q, k, v, do = inputs(1, 70, 2, 2, 64, 3)
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    gc.collect()
+    gc.disable()
+    try:
+        used = []
+        for _ in range(4):
+            torch.autograd.grad(window_attention(q, k, v, 9, 9, 1), (q, k, v), do)
+            window_attention(q, k, v, 9, 9, 1)  # a graph without a backward
+            used.append(torch.cuda.memory_allocated())
+    finally:
+        gc.enable()
+    assert used[1] == used[-1]
 
 
 @pytest.mark.gpu
