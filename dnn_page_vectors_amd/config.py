@@ -180,6 +180,8 @@ class Configuration:
             raise ValueError(f"chunk_encoder must be 'mlp' or 'cdssm', got {self.chunk_encoder!r}")
         if self.bert_window < 0 or self.bert_sinks < 0:
             raise ValueError("bert_window (0 = dense attention) and bert_sinks must be >= 0")
+        if not 0.0 <= self.bert_embed_scale < float("inf"):
+            raise ValueError(f"bert_embed_scale must be finite and >= 0 (0 = not scaled), got {self.bert_embed_scale}")
         if self.num_workers < 0 or self.prefetch < 1:
             raise ValueError("num_workers must be >= 0 (0 = auto) and prefetch >= 1")
 

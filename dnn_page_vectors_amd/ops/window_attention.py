@@ -153,8 +153,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
         raise TypeError(f"window_attention: the GPU kernels take bfloat16, got {q.dtype}")
     if d not in HEAD_DIMS:
         raise ValueError(f"window_attention: head dim must be one of {HEAD_DIMS} on the GPU, got {d}")
-    if L > MAX_LEN:
-        raise ValueError(f"window_attention: length {L} is over {MAX_LEN}")
+    if L > MAX_LEN or N * H * -(-L // 128) >= 1 << 31:
+        raise ValueError(f"window_attention: {tuple(q.shape)} is outside the kernels' range (length {MAX_LEN}, 2^31 blocks of 128 queries)")
     if q.numel() == 0:
         return q * 1.0
     return _native.binding().window_attention(q, k, v, mask, *win, scale)
@@ -222,7 +222,7 @@ def packed_window_attention(qkv: torch.Tensor, masks: Sequence[Optional[torch.Te
     _window(left, right, sinks, 1)
     masks = [_key_mask(m, N, L, qkv.device) for m, (N, L) in zip(masks, shapes)]
     if use_hip(qkv) and qkv.dtype == torch.bfloat16 and d in HEAD_DIMS and min((n for s in shapes for n in s), default=0) > 0 \
-            and qkv.data_ptr() % 16 == 0:
+            and qkv.data_ptr() % 16 == 0 and qkv.shape[1] < 1 << 24:
         train = torch.is_grad_enabled() and qkv.requires_grad
         if train:
             _native.binding().check_capture(qkv, "packed_window_attention")

@@ -76,6 +76,9 @@ def test_config_refusals_and_round_trip(tmp_path):
         Configuration(bert_window=-1)
     with pytest.raises(ValueError):
         Configuration(bert_sinks=-1)
+    for scale in (-1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            Configuration(bert_embed_scale=scale)
     cfg = config()
     cfg.save_json(str(tmp_path / "c.json"))
     back = Configuration.load_json(str(tmp_path / "c.json"))
