@@ -1,5 +1,6 @@
 """The C++ autograd binding (csrc/binding): built, loadable without a GPU, over the launchers of the library in use."""
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -44,3 +45,44 @@ def test_calls_the_debug_library(monkeypatch):
         b.init(addresses(release))
     assert torch.equal(got.q, want.q) and torch.equal(got.s, want.s)
     assert _native.binding() is b
+
+
+@pytest.mark.gpu
+def test_two_threads_on_their_own_streams():
+    """A run of the three operators from two threads at once equals the same run alone."""
+    from dnn_page_vectors_amd.ops import ckpt8
+    from dnn_page_vectors_amd.ops.embedding import scaled_embedding
+    from dnn_page_vectors_amd.ops.window_attention import window_attention
+
+    N, L, H, d = 3, 150, 2, 64
+    gen = torch.Generator().manual_seed(4)
+    ids = torch.randint(0, 500, (N, L), generator=gen).cuda()
+    W = torch.randn(500, 3 * H * d, generator=gen).cuda()
+    b = torch.randn(H * d, generator=gen).cuda()
+    do = torch.randn(N, L, H * d, generator=gen).bfloat16().cuda()
+
+    def run():
+        w, bias = W.detach().requires_grad_(), b.detach().requires_grad_()
+        q, k, v = scaled_embedding(ids, w, 0.5, 0).view(N, L, 3, H, d).unbind(2)
+        y = ckpt8.bias_gelu(window_attention(q, k, v, 20, 20, 1, ids != 0).reshape(N, L, H * d), bias)
+        return (y,) + torch.autograd.grad(y, (w, bias), do)
+
+    want = run()
+    torch.cuda.synchronize()
+    failed = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = run()
+                s.synchronize()
+                if not all(torch.equal(x, y) for x, y in zip(got, want)):
+                    failed.append(threading.get_ident())
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed

@@ -383,3 +383,24 @@ def test_nothing_outlives_its_graph():
     finally:
         gc.enable()
     assert used[1] == used[-1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [2048, 2047])
+def test_offsets_past_32_bits(D):
+    """More than 2^31 elements: the last rows equal those of a call of their own."""
+    T, tail = (1 << 31) // D + 40, 40
+    x = torch.randn(T, D, device="cuda", dtype=torch.bfloat16)
+    b = torch.randn(D, device="cuda")
+    p, q = ckpt8.pack(x), ckpt8.pack(x[-tail:].clone())
+    assert torch.equal(p.q[-tail:], q.q) and torch.equal(p.s[-tail:], q.s)
+    assert torch.equal(ckpt8.unpack(p)[-tail:], ckpt8.unpack(q))
+    del p
+    both = []
+    for t in (x, x[-tail:].clone()):
+        t.requires_grad_()
+        y = ckpt8.bias_gelu(t, b)
+        both.append((y[-tail:].clone(), torch.autograd.grad(y, t, y.detach())[0][-tail:].clone()))
+        del y
+    for u, w in zip(*both):
+        assert torch.equal(u, w)

@@ -106,6 +106,22 @@ def test_sort_of_many_tokens(T, V, E):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """More than 2^31 elements; a gradient that is zero but for the last tokens."""
+    V, E, tail = 1000, 768, 500
+    T = (1 << 31) // E + tail
+    ids = zipf(T, V, 9).int().cuda()
+    W = torch.randn(V, E, device="cuda", requires_grad=True)
+    out = scaled_embedding(ids, W, 0.5, 0)
+    assert torch.equal(out[-tail:], (W.detach()[ids[-tail:].long()] * 0.5).bfloat16())
+    g = torch.zeros_like(out)
+    g[-tail:] = torch.randn(tail, E, device="cuda").bfloat16()
+    (dW,) = torch.autograd.grad(out, W, g)
+    want, tol = grad_oracle(ids[-tail:], g[-tail:], V, 0.5, 0)
+    assert ((dW.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("E", [1021, 1024, 1028, 2500])
 @pytest.mark.parametrize("T", [100, 4000])
 def test_wide_rows(E, T):

@@ -309,6 +309,37 @@ def test_strides():
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits_by_strides():
+    """Sequences 2^31 + 64 elements apart; rows 2^24 - 8 apart, the widest that is not copied."""
+    def spread(t, step, row):
+        x = torch.empty((t.shape[0] - 1) * step + (t.shape[1] - 1) * row + t[0, 0].numel(), dtype=t.dtype, device=t.device)
+        return x.as_strided(t.shape, (step, row, *t.stride()[2:])).copy_(t)
+
+    for N, L, step, row in ((2, 150, (1 << 31) + 64, 2 * 64), (1, 131, 0, (1 << 24) - 8)):
+        q, k, v, do = inputs(N, L, 2, 2, 64, 5)
+        base = check(q, k, v, do, 30, 30, 1, None)
+        got = check(*(spread(t, step, row) for t in (q, k, v, do)), 30, 30, 1, None)
+        for x, y in zip(base, got):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits_by_length():
+    """2^31 and more elements per operand: the last rows equal those of the last tiles alone."""
+    L, H, d, tail = (1 << 20) + 300, 16, 128, 300 + 256
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randn(1, L, H, d, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(4))
+    whole = [t.requires_grad_() for t in (q, k, v)]
+    o = window_attention(*whole, 9, 5)
+    got = (o,) + torch.autograd.grad(o, whole, do)
+    part = [t.detach()[:, -tail:].contiguous().requires_grad_() for t in (q, k, v)]
+    o2 = window_attention(*part, 9, 5)
+    want = (o2,) + torch.autograd.grad(o2, part, do[:, -tail:].contiguous())
+    for x, y in zip(got, want):
+        assert torch.equal(x[:, -300:], y[:, -300:])
+
+
+@pytest.mark.gpu
 def test_same_bits_every_run_and_on_a_side_stream():
     q, k, v, do = inputs(3, 333, 4, 2, 64, 6)
     m = ragged(3, 333, 2).cuda()
