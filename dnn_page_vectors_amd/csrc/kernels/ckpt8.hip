@@ -15,8 +15,12 @@
 // arithmetic and column sums are fp32.
 //
 // A thread takes 8 consecutive columns of a row (16-byte accesses of bf16, 8-byte of q) and four
-// neighbours share a block's maximum by two lane exchanges; rows that are no multiple of 8 or not aligned
-// take the one-column-per-lane kernels, a half-wave per block.
+// neighbours share a block's maximum by two lane exchanges.  The accesses are declared with their element's
+// alignment, so rows of any length take them (global memory is read and written at any address).  The piece
+// that a row ends in (ODD: rows that are no multiple of 8) reads on into the next row and is stored by elements; only in the last rows it is read by
+// elements too.
+#include <type_traits>
+
 #include "common.h"
 
 namespace pv {
@@ -39,14 +43,27 @@ __device__ __forceinline__ float inv_pow2(int s) { return __uint_as_float((unsig
 // largest magnitude with NaN kept: the comparison of bit patterns orders |x| and puts NaN on top
 __device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2_a1 __attribute__((ext_vector_type(2), aligned(1)));
+
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const unsigned short* p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(unsigned short* p, float v) { *p = f32_to_bf16(v); }
+
+// 8 consecutive values; TAIL: n of them (n >= 8: all), zeros behind
+template <bool TAIL, typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&x)[8]) {
+  if (TAIL && n < 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? load1(p + i) : 0.f;
+  } else if constexpr (sizeof(T) == 4) {
+    const f32x4_a4 a = reinterpret_cast<const f32x4_a4*>(p)[0], b = *reinterpret_cast<const f32x4_a4*>(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
   } else {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+    const u32x4_a2 a = *reinterpret_cast<const u32x4_a2*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[2 * i] = __uint_as_float(a[i] << 16);
@@ -55,24 +72,39 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
   }
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+__device__ __forceinline__ void store8(T* p, int n, const float (&x)[8]) {
+  if (n < 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) store1(p + i, x[i]);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4_a4*>(p) = f32x4_a4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4_a4*>(p + 4) = f32x4_a4{x[4], x[5], x[6], x[7]};
   } else {
-    *reinterpret_cast<u32x4*>(p) =
-        u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    *reinterpret_cast<u32x4_a2*>(p) =
+        u32x4_a2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
   }
 }
-template <typename T>
-__device__ __forceinline__ float load1(const T* p) {
-  if constexpr (sizeof(T) == 4) return *p;
-  else return bf16_to_f32(*p);
+template <bool TAIL>
+__device__ __forceinline__ u32x2 load_bytes(const unsigned char* p, int n) {
+  if (!TAIL || n >= 8) {
+    const u32x2_a1 w = *reinterpret_cast<const u32x2_a1*>(p);
+    return u32x2{w[0], w[1]};
+  }
+  u32x2 w{0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < n) w[i / 4] |= (unsigned)p[i] << (8 * (i % 4));
+  return w;
 }
-template <typename T>
-__device__ __forceinline__ void store1(T* p, float v) {
-  if constexpr (sizeof(T) == 4) *p = v;
-  else *p = f32_to_bf16(v);
+__device__ __forceinline__ void store_bytes(unsigned char* p, int n, u32x2 w) {
+  if (n >= 8) {
+    *reinterpret_cast<u32x2_a1*>(p) = u32x2_a1{w[0], w[1]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) p[i] = (unsigned char)(w[i / 4] >> (8 * (i % 4)));
+  }
 }
 
 // 8 values / 2^(s-127) -> e4m3 bytes (round to nearest even)
@@ -120,38 +152,49 @@ struct Shape {
   int tpr, rpb;  // rpb = rows per workgroup
 };
 struct Place {
-  int c, sub, step;
+  int c, n, sub, step;  // n = columns from c to the row's end
   long r0, r1;
   bool on;
 };
+template <bool ODD>
 __device__ __forceinline__ Place place(const Shape& s) {
   Place p;
   p.sub = threadIdx.x / s.tpr;
   p.c = blockIdx.y * 2048 + (threadIdx.x - p.sub * s.tpr) * 8;
+  p.n = ODD ? s.D - p.c : 8;
   p.step = 256 / s.tpr;
   p.r0 = (long)blockIdx.x * s.rpb + p.sub;
   p.r1 = min(s.T, (long)(blockIdx.x + 1) * s.rpb);
   p.on = p.sub < p.step && p.c < s.D;
   return p;
 }
+// body(first row, TAIL) over the workgroup's rows, U passes at a time; TAIL where a row's last piece may read behind
+// the last row of all (8 columns are at most 8 rows)
+template <int U, bool ODD, typename F>
+__device__ __forceinline__ void each_rows(const Shape& s, const Place& p, F body) {
+  for (long r = p.r0; r < p.r1; r += U * p.step) {
+    if (ODD && r - p.sub + U * p.step + 8 >= s.T) body(r, std::true_type());
+    else body(r, std::false_type());
+  }
+}
 
 // MODE 0: pack x;  1: u = x + b, y = gelu(u), pack u.  U rows in flight per thread.
-template <typename T, int MODE, int U>
+template <typename T, int MODE, int U, bool ODD>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, const float* __restrict__ b,
                                                    T* __restrict__ y, unsigned char* __restrict__ q,
                                                    unsigned char* __restrict__ sc, Shape s) {
-  const Place p = place(s);
+  const Place p = place<ODD>(s);
   float bias[8];
   if constexpr (MODE == 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bias[i] = p.on ? b[p.c + i] : 0.f;
+    for (int i = 0; i < 8; ++i) bias[i] = p.on && i < p.n ? b[p.c + i] : 0.f;
   }
-  for (long r = p.r0; r < p.r1; r += U * p.step) {  // lanes that share a block leave together: same sub
+  each_rows<U, ODD>(s, p, [&](long r, auto tail) {  // lanes that share a block leave together: same sub
     float v[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long rr = min(r + u * p.step, p.r1 - 1);
-      if (p.on) load8(x + rr * s.D + p.c, v[u]);
+      if (p.on) load8<tail>(x + rr * s.D + p.c, p.n, v[u]);
       else
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
@@ -164,62 +207,37 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, cons
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (MODE == 1) v[u][i] += bias[i];
+        v[u][i] = i < p.n ? v[u][i] : 0.f;  // what lies behind the row
         m = max(m, mag(v[u][i]));
       }
       m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
       m = max(m, (unsigned)__shfl_xor((int)m, 2, 64));
       if (!p.on) continue;
       const int e = scale_byte(__uint_as_float(m));
-      *reinterpret_cast<u32x2*>(q + rr * s.D + p.c) = quant8(v[u], e);
+      store_bytes(q + rr * s.D + p.c, p.n, quant8(v[u], e));
       if ((p.c & 31) == 0) sc[rr * s.nb + p.c / BLK] = (unsigned char)e;
       if constexpr (MODE == 1) {
         float o[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = v[u][i] * sig(v[u][i]);
-        store8(y + rr * s.D + p.c, o);
+        store8(y + rr * s.D + p.c, p.n, o);
       }
     }
-  }
+  });
 }
 
-// the same for any D and alignment: a half-wave per block of 32 columns
-template <typename T, int MODE>
-__global__ __launch_bounds__(256) void pack_any_kernel(const T* __restrict__ x, const float* __restrict__ b,
-                                                       T* __restrict__ y, unsigned char* __restrict__ q,
-                                                       unsigned char* __restrict__ sc, Shape s) {
-  const long blocks = s.T * s.nb, step = (long)gridDim.x * 8;
-  const int lane = threadIdx.x & 31;
-  for (long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5); i < blocks; i += step) {
-    const long r = i / s.nb;
-    const int blk = (int)(i - r * s.nb), c = blk * BLK + lane;
-    const bool on = c < s.D;
-    float v = on ? load1(x + r * s.D + c) : 0.f;
-    if constexpr (MODE == 1) v += on ? b[c] : 0.f;
-    unsigned m = mag(v);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-    const int e = scale_byte(__uint_as_float(m));
-    if (on) {
-      const int w = e == 255 ? 0x7F : __builtin_amdgcn_cvt_pk_fp8_f32(v * inv_pow2(e), 0.f, 0, false);
-      q[r * s.D + c] = (unsigned char)w;
-      if (MODE == 1) store1(y + r * s.D + c, v * sig(v));
-    }
-    if (lane == 0) sc[r * s.nb + blk] = (unsigned char)e;
-  }
-}
-
-template <typename T, int U>
+template <typename T, int U, bool ODD>
 __global__ __launch_bounds__(256) void unpack_kernel(const unsigned char* __restrict__ q,
                                                      const unsigned char* __restrict__ sc, T* __restrict__ x, Shape s) {
-  const Place p = place(s);
+  const Place p = place<ODD>(s);
   if (!p.on) return;
-  for (long r = p.r0; r < p.r1; r += U * p.step) {
+  each_rows<U, ODD>(s, p, [&](long r, auto tail) {
     u32x2 w[U];
     int e[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long rr = min(r + u * p.step, p.r1 - 1);
-      w[u] = *reinterpret_cast<const u32x2*>(q + rr * s.D + p.c);
+      w[u] = load_bytes<tail>(q + rr * s.D + p.c, p.n);
       e[u] = sc[rr * s.nb + p.c / BLK];
     }
 #pragma unroll
@@ -228,26 +246,13 @@ __global__ __launch_bounds__(256) void unpack_kernel(const unsigned char* __rest
       if (rr >= p.r1) break;
       float v[8];
       dequant8(w[u], e[u], v);
-      store8(x + rr * s.D + p.c, v);
+      store8(x + rr * s.D + p.c, p.n, v);
     }
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void unpack_any_kernel(const unsigned char* __restrict__ q,
-                                                         const unsigned char* __restrict__ sc, T* __restrict__ x,
-                                                         Shape s) {
-  const long n = s.T * s.D, step = (long)gridDim.x * 256;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const long r = i / s.D;
-    const int c = (int)(i - r * s.D);
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], false);
-    store1(x + i, a[0] * scale_of(sc[r * s.nb + c / BLK]));
-  }
+  });
 }
 
 // du = dy gelu'(u^) -> dx, column partials of this workgroup's rows -> part[blockIdx.x][D]; Y: y^ = gelu(u^) too
-template <int U, bool Y>
+template <int U, bool Y, bool ODD>
 __global__ __launch_bounds__(256) void gelu_bwd_kernel(const unsigned char* __restrict__ q,
                                                        const unsigned char* __restrict__ sc,
                                                        const unsigned short* __restrict__ dy,
@@ -255,20 +260,20 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const unsigned char* __re
                                                        unsigned short* __restrict__ yh, float* __restrict__ part,
                                                        Shape s) {
   __shared__ __attribute__((aligned(16))) float sh[256 * 8];
-  const Place p = place(s);
+  const Place p = place<ODD>(s);
   float acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
   if (p.on)
-    for (long r = p.r0; r < p.r1; r += U * p.step) {
+    each_rows<U, ODD>(s, p, [&](long r, auto tail) {
       u32x2 w[U];
-      u32x4 gv[U];
+      float gv[U][8];
       int e[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long rr = min(r + u * p.step, p.r1 - 1);
-        w[u] = *reinterpret_cast<const u32x2*>(q + rr * s.D + p.c);
-        gv[u] = *reinterpret_cast<const u32x4*>(dy + rr * s.D + p.c);
+        w[u] = load_bytes<tail>(q + rr * s.D + p.c, p.n);
+        load8<tail>(dy + rr * s.D + p.c, p.n, gv[u]);
         e[u] = sc[rr * s.nb + p.c / BLK];
       }
 #pragma unroll
@@ -279,16 +284,15 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const unsigned char* __re
         dequant8(w[u], e[u], v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float g = (i & 1) ? __uint_as_float(gv[u][i / 2] & 0xFFFF0000u) : __uint_as_float(gv[u][i / 2] << 16);
           const float sg = sig(v[i]);
-          d[i] = g * slope(v[i], sg);
+          d[i] = gv[u][i] * slope(v[i], sg);
           acc[i] += d[i];
           o[i] = v[i] * sg;
         }
-        store8(dx + rr * s.D + p.c, d);
-        if constexpr (Y) store8(yh + rr * s.D + p.c, o);
+        store8(dx + rr * s.D + p.c, p.n, d);
+        if constexpr (Y) store8(yh + rr * s.D + p.c, p.n, o);
       }
-    }
+    });
   // rows of the workgroup's passes: sub 0 adds the others in order
 #pragma unroll
   for (int i = 0; i < 8; ++i) sh[threadIdx.x * 8 + i] = acc[i];
@@ -297,39 +301,8 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const unsigned char* __re
     for (int k = 1; k < p.step; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] += sh[(k * s.tpr + threadIdx.x) * 8 + i];
-    float* pr = part + (size_t)blockIdx.x * s.D + p.c;
-    reinterpret_cast<f32x4*>(pr)[0] = f32x4{acc[0], acc[1], acc[2], acc[3]};
-    reinterpret_cast<f32x4*>(pr)[1] = f32x4{acc[4], acc[5], acc[6], acc[7]};
+    store8(part + (size_t)blockIdx.x * s.D + p.c, p.n, acc);
   }
-}
-
-// any D and alignment: a thread owns one column of rpb rows (grid.y = column blocks of 64, 4 row lanes)
-template <bool Y>
-__global__ __launch_bounds__(256) void gelu_bwd_any_kernel(const unsigned char* __restrict__ q,
-                                                           const unsigned char* __restrict__ sc,
-                                                           const unsigned short* __restrict__ dy,
-                                                           unsigned short* __restrict__ dx,
-                                                           unsigned short* __restrict__ yh, float* __restrict__ part,
-                                                           Shape s) {
-  __shared__ float sh[4][64];
-  const int c = blockIdx.y * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
-  const long r1 = min(s.T, (long)(blockIdx.x + 1) * s.rpb);
-  float acc = 0.f;
-  if (c < s.D) {
-#pragma unroll 4
-    for (long r = (long)blockIdx.x * s.rpb + sub; r < r1; r += 4) {
-      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[r * s.D + c], false);
-      const float v = a[0] * scale_of(sc[r * s.nb + c / BLK]);
-      const float sg = sig(v), d = bf16_to_f32(dy[r * s.D + c]) * slope(v, sg);
-      acc += d;
-      dx[r * s.D + c] = f32_to_bf16(d);
-      if constexpr (Y) yh[r * s.D + c] = f32_to_bf16(v * sg);
-    }
-  }
-  sh[sub][threadIdx.x & 63] = acc;
-  __syncthreads();
-  if (sub == 0 && c < s.D)
-    part[(size_t)blockIdx.x * s.D + c] = ((sh[0][threadIdx.x] + sh[1][threadIdx.x]) + sh[2][threadIdx.x]) + sh[3][threadIdx.x];
 }
 
 // out[c] (+)= sum of the S partial rows, in row order within each of the 16 row lanes, then over the lanes
@@ -351,10 +324,6 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
   }
 }
 
-__host__ inline bool vec_ok(int D, const void* a, const void* b, const void* c, const void* d) {
-  const size_t m = (size_t)a | (size_t)b | (size_t)c | (size_t)d;
-  return D % 8 == 0 && (m & 15) == 0;
-}
 __host__ inline Shape shape(long T, int D, long want) {
   Shape s{};
   s.T = T;
@@ -385,13 +354,9 @@ template <typename T, int MODE>
 int pack(const T* x, const float* b, T* y, unsigned char* q, unsigned char* sc, long rows, int D, hipStream_t st) {
   if (rows == 0) return 0;
   const Shape s = shape(rows, D, many(rows, D));
-  if (vec_ok(D, x, y, q, nullptr)) {
-    const dim3 grid((unsigned)((rows + s.rpb - 1) / s.rpb), cols(D));
-    hipLaunchKernelGGL((pack_kernel<T, MODE, 4>), grid, dim3(256), 0, st, x, b, y, q, sc, s);
-  } else {
-    const long n = (rows * s.nb + 7) / 8;
-    hipLaunchKernelGGL((pack_any_kernel<T, MODE>), dim3((unsigned)min(n, 16384L)), dim3(256), 0, st, x, b, y, q, sc, s);
-  }
+  const dim3 grid((unsigned)((rows + s.rpb - 1) / s.rpb), cols(D));
+  if (D % 8) hipLaunchKernelGGL((pack_kernel<T, MODE, 4, true>), grid, dim3(256), 0, st, x, b, y, q, sc, s);
+  else hipLaunchKernelGGL((pack_kernel<T, MODE, 4, false>), grid, dim3(256), 0, st, x, b, y, q, sc, s);
   PV_LAUNCH_CHECK();
   return 0;
 }
@@ -400,13 +365,9 @@ template <typename T>
 int unpack(const unsigned char* q, const unsigned char* sc, T* x, long rows, int D, hipStream_t st) {
   if (rows == 0) return 0;
   const Shape s = shape(rows, D, many(rows, D));
-  if (vec_ok(D, x, q, nullptr, nullptr)) {
-    const dim3 grid((unsigned)((rows + s.rpb - 1) / s.rpb), cols(D));
-    hipLaunchKernelGGL((unpack_kernel<T, 4>), grid, dim3(256), 0, st, q, sc, x, s);
-  } else {
-    const long n = (rows * (long)D + 255) / 256;
-    hipLaunchKernelGGL((unpack_any_kernel<T>), dim3((unsigned)min(n, 16384L)), dim3(256), 0, st, q, sc, x, s);
-  }
+  const dim3 grid((unsigned)((rows + s.rpb - 1) / s.rpb), cols(D));
+  if (D % 8) hipLaunchKernelGGL((unpack_kernel<T, 4, true>), grid, dim3(256), 0, st, q, sc, x, s);
+  else hipLaunchKernelGGL((unpack_kernel<T, 4, false>), grid, dim3(256), 0, st, q, sc, x, s);
   PV_LAUNCH_CHECK();
   return 0;
 }
@@ -452,21 +413,14 @@ PV_API int pv_ckpt8_gelu_bwd(const void* q, const void* s, const void* dy, void*
   const unsigned char *qq = (const unsigned char*)q, *ss = (const unsigned char*)s;
   const unsigned short* g = (const unsigned short*)dy;
   unsigned short *d = (unsigned short*)dx, *y = (unsigned short*)yh;
-  const bool vec = vec_ok(D, q, dy, dx, yh) && ((size_t)ws & 15) == 0;
-  Shape p = shape(T, D, groups(T));
-  if (!vec) p.rpb = (int)((T + groups(T) - 1) / groups(T));
+  const Shape p = shape(T, D, groups(T));
   const int S = T ? (int)((T + p.rpb - 1) / p.rpb) : 0;
-  float* part = (S == 1 && !db_add && ((size_t)db & 15) == 0) ? db : ws;  // one row group: its sums are the result
+  float* part = S == 1 && !db_add ? db : ws;  // one row group: its sums are the result
   if (S) {
-    if (vec) {
-      const dim3 grid(S, cols(D));
-      if (y) hipLaunchKernelGGL((gelu_bwd_kernel<4, true>), grid, dim3(256), 0, st, qq, ss, g, d, y, part, p);
-      else hipLaunchKernelGGL((gelu_bwd_kernel<4, false>), grid, dim3(256), 0, st, qq, ss, g, d, y, part, p);
-    } else {
-      const dim3 grid(S, (D + 63) / 64);
-      if (y) hipLaunchKernelGGL((gelu_bwd_any_kernel<true>), grid, dim3(256), 0, st, qq, ss, g, d, y, part, p);
-      else hipLaunchKernelGGL((gelu_bwd_any_kernel<false>), grid, dim3(256), 0, st, qq, ss, g, d, y, part, p);
-    }
+    const dim3 grid(S, cols(D));
+    const auto kernel = D % 8 ? (y ? gelu_bwd_kernel<4, true, true> : gelu_bwd_kernel<4, false, true>)
+                              : (y ? gelu_bwd_kernel<4, true, false> : gelu_bwd_kernel<4, false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, qq, ss, g, d, y, part, p);
     PV_LAUNCH_CHECK();
   }
   if (part != db) {
