@@ -74,7 +74,8 @@ __device__ __forceinline__ void store8(unsigned short* p, const float (&x)[8]) {
 // ------------------------------------------------------------------------------------ lookup
 // A workgroup owns `rows` consecutive tokens; a thread takes pieces of C columns of them, four at a time so that
 // four rows are on their way at once (C = 8: 16-byte stores; C = 1: row lengths or pointers that are no
-// multiple of 16 bytes).
+// multiple of 16 bytes).  73728 tokens x 768 fp32 -> bf16: 42 us (2.7 TB/s written, 5.4 read, the table from the
+// caches); 256000 x 512: 82 us.
 template <typename TW, typename TO, int C>
 __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restrict__ W, TO* __restrict__ out, long T,
                                                      long V, int E, float scale, int rows,
@@ -377,7 +378,9 @@ __global__ __launch_bounds__(TILE) void place_kernel(Tokens<KT> src, long T, lon
   }
 }
 
-// A wave adds the rows of its chunk of the sorted tokens, run by run.  Partial rows: slot 2 c = the
+// A wave adds the rows of its chunk of the sorted tokens, run by run (bound by the rows' reads, 512 bytes each at
+// their tokens' places: 42 us at 73728 tokens x 768, 84 at 256000 x 512; chunks of 16 tokens 137 and 251 us instead of 125
+// and 217 for the whole, of 64 tokens 149 and 221).  Partial rows: slot 2 c = the
 // part of a run that began before chunk c, slot 2 c + 1 = the part of a run that begins in chunk c
 // and goes on behind it.
 template <typename TG, typename KT, int W>

@@ -382,7 +382,11 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
 
 // ------------------------------------------------------------------------------------ forward
 // Workgroup = 128 queries of one head; a wave owns 32 of them (lane & 31), both half-waves hold the
-// same queries and split the keys of each block.
+// same queries and split the keys of each block.  Bound by instruction issue, vector and matrix about equally:
+// 12 heads x 64, 32 ragged pages x 2000 tokens, window 256 + 256: 173 - 187 us (about 400 TFLOP/s of visible pairs, no
+// rescaling of accumulators in nearly all blocks); all 2048 x 2048 pairs 500 - 590 us (820 - 700); 16 heads x 128,
+// 4 x 4096 causal, window 1024: 195 - 216 (600).  Workgroups of 8 waves read the keys half as often and took 229
+// against 187 us; 64 queries per wave 242 against 181 (registers).
 template <int D>
 __global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short kt[2][TK * D];
@@ -468,7 +472,9 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
 
 // ------------------------------------------------------------------------------------ backward: dq, D
 // Same walk as the forward: dS^T in registers, dq^T += K^T dS^T.  D is the lane's own row sum of
-// do * o and goes to memory for the other kernel; -D is the start value of the dP accumulators.
+// do * o and goes to memory for the other kernel; -D is the start value of the dP accumulators (from zero,
+// subtracted later: 623 instead of 618 us, forward and backward of the forward's pages).  Those pages:
+// 229 - 267 us; four waves per SIMD spill and cost 35 us.
 template <int D>
 __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short kt[2][TK * D];
@@ -547,7 +553,9 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
 // ------------------------------------------------------------------------------------ backward: dk, dv
 // Workgroup = 128 keys of one key/value head, a wave owns 32 of them; it walks the query tiles of
 // every query head of the group: P and dS (queries x keys), dv^T += dO^T P, dk^T += Q^T dS.  The rows'
-// -D are the start values of the dP accumulators, read from LDS into place.
+// -D are the start values of the dP accumulators, read from LDS into place.  The forward's pages: 296 - 303 us with
+// the far queries; heads of 128: one wave per SIMD (321 registers), 426 - 446 us, and a tile's two blocks taken
+// together, products under exponentials, need more than 512 (spills: 741 -> 976 us, forward and backward).
 //
 // The sinks are seen by every later query: walked by their own workgroup alone they would make it the last
 // by far.  Their far queries (behind the window's tiles) are dealt to workgroups of FAR tiles each, whose
@@ -792,8 +800,9 @@ __host__ inline int check_sizes(long N, long L, long H, long G, int d, float sca
 }
 
 // The far part of the sinks is split off where they all lie in the first workgroup of keys and it is long
-// enough to matter (8 tiles: a window's own walk at left + right = 384).  More sinks than that fill several
-// workgroups with long walks, which balance among themselves.
+// enough to matter (8 tiles; forward and backward of 64 pages x 12 heads x 64, window 128 + 128, one sink, split / not:
+// 5 tiles behind the window 356 / 352 us, 9 tiles 484 / 484, 15 tiles 682 / 715; 2 pages of 4096: 117 / 200).  More
+// sinks than that fill several workgroups with long walks, which balance among themselves.
 struct FarPlan {
   int wgs, chunks, blocks, tile;
   long near_slots, floats;
