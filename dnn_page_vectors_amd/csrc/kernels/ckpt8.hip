@@ -18,8 +18,8 @@
 // neighbours share a block's maximum by two lane exchanges.  The accesses are declared with their element's
 // alignment, so rows of any length take them (global memory is read and written at any address).  The piece
 // that a row ends in (ODD: rows that are no multiple of 8, kernels of their own for their registers: with the tail
-// code in, 73728 x 2048 bias + GELU took 328 us instead of 317) reads on into the next row and is stored by elements; only in the last rows it is read by
-// elements too.
+// code in, 73728 x 2048 bias + GELU took 328 us instead of 317) reads on into the next row and is stored by
+// elements; only in the last rows it is read by elements too.
 #include <type_traits>
 
 #include "common.h"

@@ -10,8 +10,8 @@
 // ids (a word of a Zipf text is several percent of all tokens).  Here every row has one writer:
 //   * few tokens (T <= SMALL_T): one launch.  A workgroup per token; the first token of an id adds
 //     all rows of that id, found by comparing ids; other workgroups zero the rows without a token.
-//   * else the tokens are sorted by id (two launches per 8 bits, which zero the gradient on the way; stable), a wave adds the rows of CHUNK
-//     consecutive sorted tokens, writing the runs that lie inside its chunk, and the runs that
+//   * else the tokens are sorted by id (two launches per 8 bits, which zero the gradient on the way; stable), a wave
+//     adds the rows of CHUNK consecutive sorted tokens, writing the runs that lie inside its chunk, and the runs that
 //     cross a chunk's border are joined from the chunks' fp32 partial rows by a second launch.
 // All sums are fp32, in an order that depends on the sizes and ids alone.
 #include "common.h"
@@ -52,29 +52,34 @@ __device__ __forceinline__ float load1<unsigned short>(const unsigned short* p) 
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(unsigned short* p, float v) { *p = f32_to_bf16(v); }
 
+// Vectors of the element's alignment: global memory is read and written at any address, rows of any length take them
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+  const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(p), b = *reinterpret_cast<const f32x4_a4*>(p + 4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
 }
 __device__ __forceinline__ void load8(const unsigned short* p, float (&x)[8]) {
-  const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+  const u32x4_a2 a = *reinterpret_cast<const u32x4_a2*>(p);
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(a[i] << 16), x[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
 }
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-  reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+  *reinterpret_cast<f32x4_a4*>(p) = f32x4_a4{x[0], x[1], x[2], x[3]};
+  *reinterpret_cast<f32x4_a4*>(p + 4) = f32x4_a4{x[4], x[5], x[6], x[7]};
 }
 __device__ __forceinline__ void store8(unsigned short* p, const float (&x)[8]) {
-  *reinterpret_cast<u32x4*>(p) =
-      u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+  *reinterpret_cast<u32x4_a2*>(p) =
+      u32x4_a2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
 }
 
 // ------------------------------------------------------------------------------------ lookup
 // A workgroup owns `rows` consecutive tokens; a thread takes pieces of C columns of them, four at a time so that
-// four rows are on their way at once (C = 8: 16-byte stores; C = 1: row lengths or pointers that are no
-// multiple of 16 bytes).  73728 tokens x 768 fp32 -> bf16: 42 us (2.7 TB/s written, 5.4 read, the table from the
+// four rows are on their way at once.  C = 8: a row's last piece is its last 8 columns, which two threads may write
+// alike; C = 1: rows of fewer columns (a column per thread took 106 us instead of 37 at 73728 x 767).  73728 tokens x 768 fp32 -> bf16: 42 us (2.7 TB/s written, 5.4 read, the table from the
 // caches); 256000 x 512: 82 us.
 template <typename TW, typename TO, int C>
 __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restrict__ W, TO* __restrict__ out, long T,
@@ -82,7 +87,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restri
                                                      const float* __restrict__ pos, const float* __restrict__ typ,
                                                      Groups gr) {
   const long t0 = (long)blockIdx.x * rows;
-  const int n = (int)min((long)rows, T - t0), per = E / C, all = n * per;
+  const int n = (int)min((long)rows, T - t0), per = (E + C - 1) / C, all = n * per;
   for (int x0 = threadIdx.x; x0 < all; x0 += 1024) {
     int r[4], c[4];
     long id[4];
@@ -91,7 +96,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restri
     for (int u = 0; u < 4; ++u) {
       const int x = min(x0 + 256 * u, all - 1);
       r[u] = x / per;
-      c[u] = (x - r[u] * per) * C;
+      c[u] = min((x - r[u] * per) * C, E - C);
       id[u] = ids.at(t0 + r[u]);
     }
 #pragma unroll
@@ -121,9 +126,12 @@ __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restri
 }
 
 // ------------------------------------------------------------------------------------ gradient
-// A lane owns W consecutive columns (4, or 1 where rows are not 4-aligned) of a slab of 64 W columns (grid.y).
+// A lane owns W consecutive columns (4, or 1 of rows with fewer than 4) of a slab of 64 W columns (grid.y).
 // One slab per wave: a wave over a whole row of 768 has a third of the waves and as many loads under way
 // (walk_kernel 87 us instead of 44 at 73728 tokens x 768).
+// Where a row is no multiple of 4, the lane that it ends in takes the row's last 4 columns: those that it shares with its
+// neighbour come out the same in both, and both write them, but where the row is added to (a column per lane: 126 us
+// instead of 70 for the gradient of 73728 tokens x 767).
 template <typename TG, int W>
 struct Cols {
   float a[W];
@@ -139,11 +147,11 @@ struct Cols {
     } else if constexpr (W == 1) {
       a[0] = load1(row + c);
     } else if constexpr (sizeof(TG) == 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(row + c);
+      const f32x4_a4 v = *reinterpret_cast<const f32x4_a4*>(row + min(c, E - 4));
 #pragma unroll
       for (int i = 0; i < W; ++i) a[i] = v[i];
     } else {
-      const u32x2 v = *reinterpret_cast<const u32x2*>(row + c);
+      const u32x2_a2 v = *reinterpret_cast<const u32x2_a2*>(row + min(c, E - 4));
       a[0] = __uint_as_float(v[0] << 16);
       a[1] = __uint_as_float(v[0] & 0xFFFF0000u);
       a[2] = __uint_as_float(v[1] << 16);
@@ -162,10 +170,18 @@ struct Cols {
     if constexpr (W == 1) {
       row[c] = (acc ? row[c] : 0.f) + a[0] * scale;
     } else {
-      f32x4 v = acc ? *reinterpret_cast<const f32x4*>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+      const int at = min(c, E - 4);
+      if (acc && at < c) {
+#pragma unroll
+        for (int i = 1; i < W; ++i)
+          if (at + i >= c) row[at + i] += a[i] * scale;
+        return;
+      }
+      f32x4_a4 v{0.f, 0.f, 0.f, 0.f};
+      if (acc) v = *reinterpret_cast<const f32x4_a4*>(row + at);
 #pragma unroll
       for (int i = 0; i < W; ++i) v[i] += a[i] * scale;
-      *reinterpret_cast<f32x4*>(row + c) = v;
+      *reinterpret_cast<f32x4_a4*>(row + at) = v;
     }
   }
 };
@@ -240,11 +256,9 @@ __global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __re
   for (int r = wave; r < n; r += 4) {
     if (has[r]) continue;
     float* row = dW + (r0 + r) * E;
-    if constexpr (W == 4) {
-      for (int c = lane * 4; c < E; c += 256) *reinterpret_cast<f32x4*>(row + c) = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else {
-      for (int c = lane; c < E; c += 64) row[c] = 0.f;
-    }
+    const int whole = W == 4 ? E / 4 * 4 : 0;
+    for (int c = lane * 4; c < whole; c += 256) *reinterpret_cast<f32x4_a4*>(row + c) = f32x4_a4{0.f, 0.f, 0.f, 0.f};
+    for (int c = whole + lane; c < E; c += 64) row[c] = 0.f;
   }
 }
 
@@ -575,16 +589,15 @@ int grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad
 template <typename TG>
 int grad_w(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad, float scale, int acc, char* ws,
            long ws_bytes, hipStream_t st) {
-  const bool vec = E % 4 == 0 && ((size_t)g % (4 * sizeof(TG))) == 0 && ((size_t)dW % 16) == 0;
-  return vec ? grad<TG, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st)
-             : grad<TG, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
+  return E < 4 ? grad<TG, 1>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st)
+               : grad<TG, 4>(ids, g, dW, T, V, E, pad, scale, acc, ws, ws_bytes, st);
 }
 
 template <typename TW, typename TO>
 int lookup(const Ids& ids, const TW* W, TO* out, long T, long V, int E, float scale, const float* pos,
            const float* typ, const Groups& gr, hipStream_t st) {
-  const bool vec = E % 8 == 0 && ((size_t)W % 16) == 0 && ((size_t)out % 16) == 0;
-  const int per = vec ? E / 8 : E;
+  const bool vec = E >= 8;
+  const int per = vec ? (E + 7) / 8 : E;
   const int rows = max(1, min(64, 1024 / per));  // about four pieces per thread
   const dim3 grid((unsigned)((T + rows - 1) / rows));
   if (vec)

@@ -212,6 +212,24 @@ def test_adds_into_the_flat_gradient(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [700, 6000])
+@pytest.mark.parametrize("E", [2, 5, 7, 257, 258, 259])
+def test_odd_rows_written_and_added_to(T, E):
+    """Rows whose last piece overlaps its neighbour's, across a slab's border too: written, and added into."""
+    from dnn_page_vectors_amd.ops.embedding import sorted_row_grad
+
+    V = 90
+    ids = zipf(T, V - 20, E)
+    _, g, _ = check(ids, V, E, torch.float32, 0, scale=1.5, seed=E)
+    want, tol = grad_oracle(ids, g, V, 1.5, 0)
+    room = torch.full((V * E + 2,), 0.25, device="cuda")
+    sorted_row_grad(ids.cuda(), g, room[1:-1].view(V, E), 1.5, 0, accumulate=True)
+    got = room[1:-1].view(V, E).double().cpu()
+    assert ((got - want - 0.25).abs() <= tol + 2.0 ** -24 * (want.abs() + 0.25)).all()
+    assert room[0] == 0.25 and room[-1] == 0.25 and (got[V - 20:] == 0.25).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [400, 5000])
 def test_graph_replays_and_side_stream(T):
     V, E = 900, 100
