@@ -79,7 +79,8 @@ __device__ __forceinline__ void store8(unsigned short* p, const float (&x)[8]) {
 // ------------------------------------------------------------------------------------ lookup
 // A workgroup owns `rows` consecutive tokens; a thread takes pieces of C columns of them, four at a time so that
 // four rows are on their way at once.  C = 8: a row's last piece is its last 8 columns, which two threads may write
-// alike; C = 1: rows of fewer columns (a column per thread took 106 us instead of 37 at 73728 x 767).  73728 tokens x 768 fp32 -> bf16: 42 us (2.7 TB/s written, 5.4 read, the table from the
+// alike; C = 1: rows of fewer columns (a column per thread took 106 us instead of 37 at 73728 x 767).
+// 73728 tokens x 768 fp32 -> bf16: 42 us (2.7 TB/s written, 5.4 read, the table from the
 // caches); 256000 x 512: 82 us.
 template <typename TW, typename TO, int C>
 __global__ __launch_bounds__(256) void lookup_kernel(Ids ids, const TW* __restrict__ W, TO* __restrict__ out, long T,
