@@ -27,8 +27,8 @@ namespace pv {
 namespace wattn {
 
 constexpr int TK = 64;   // rows per staged tile
-constexpr int NTH = 256;
-constexpr int RB = 128;  // rows a workgroup owns: 4 waves x 32
+constexpr int RB = 128;  // rows a workgroup owns: 4 waves x 32 (sequences up to SHORT: 2 waves, all rows)
+constexpr int SHORT = TK;
 // Query tiles per workgroup of the sinks' far part (4: 454 us instead of 448 for forward and backward of 64 pages x
 // 975 tokens x 12 heads, 755 instead of 739 for 4 x 4096 x 16 of 128).
 constexpr int FAR = 16;
@@ -103,13 +103,13 @@ __device__ __forceinline__ unsigned lds_at(const void* p) {
 }
 
 // Tile rows go from memory straight to LDS (global_load_lds_dwordx4: 64 lanes x 16 bytes land in 1 KB in
-// lane order), D / 32 pieces per wave; the swizzle is applied to the source column.
+// lane order), D / 8 pieces, W waves; the swizzle is applied to the source column.
 // In asm: for the builtin the compiler waits for every load under way before it reads any LDS of the same array,
 // which would make the prefetch of the next tile a wait for it.  No register is written; landed() and a
 // barrier stand between these loads and the reads of their tile.
-template <int D>
+template <int D, int W>
 struct Loader {
-  static constexpr int P = D / 32, RP = 512 / D;  // pieces per wave, rows per piece
+  static constexpr int P = D / (8 * W), RP = 512 / D;  // pieces per wave, rows per piece
   static constexpr int KINDS = RP % 8 ? 2 : 1;     // swz repeats every 8 rows: pieces of 4 rows come in two kinds
   static constexpr unsigned TILE = TK * D * 2;     // bytes
   unsigned off[KINDS];                              // this lane's source offset within a piece (bytes)
@@ -166,11 +166,11 @@ __device__ __forceinline__ void operands_here() {
 
 // Masked rows become zeros, so whatever they hold (infinities and NaN too) never meets a zero
 // probability in a product.  Uniform over the workgroup; ends with a barrier.
-template <int D>
+template <int D, int W>
 __device__ __forceinline__ void clear_rows(unsigned short* k, unsigned short* v, unsigned long long keep) {
 #pragma unroll
-  for (int u = 0; u < D / 32; ++u) {
-    const int c = threadIdx.x + NTH * u, r = c / (D / 8);
+  for (int u = 0; u < D / (8 * W); ++u) {
+    const int c = threadIdx.x + 64 * W * u, r = c / (D / 8);
     if (!((keep >> r) & 1ull)) {
       *reinterpret_cast<u32x4*>(k + c * 8) = u32x4{0, 0, 0, 0};
       *reinterpret_cast<u32x4*>(v + c * 8) = u32x4{0, 0, 0, 0};
@@ -293,14 +293,14 @@ struct Where {
 // Walks the key tiles that queries b0 .. b0 + RB - 1 see (the tiles of the sinks, then the window's):
 // `each(tile K, tile V, first key, keep bits)`.  While a tile is worked on, the next one is on its way to the
 // other buffer.  The mask is read ahead for 128 tiles at once, as one word per tile in LDS: tiles without
-// a key that counts cost nothing (a page's padding is such a run of tiles).
-template <int D, typename F>
-__device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0, unsigned short (&kt)[2][TK * D],
-                                          unsigned short (&vt)[2][TK * D], unsigned long long (&words)[128], F each) {
+// a key that counts cost nothing (a page's padding is such a run of tiles).  B = 1: there is one tile only.
+template <int D, int W, int B, typename F>
+__device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0, unsigned short (&kt)[B][TK * D],
+                                          unsigned short (&vt)[B][TK * D], unsigned long long (&words)[128], F each) {
   const int lane = threadIdx.x & 63;
   const unsigned short* K = a.k.p + n * a.k.n + kvh * a.k.h;
   const unsigned short* V = a.v.p + n * a.v.n + kvh * a.v.h;
-  Loader<D> lk, lv;
+  Loader<D, W> lk, lv;
   lk.init(K, a.k.l, kt[0]);
   lv.init(V, a.v.l, vt[0]);
   const int lo = max(0, b0 - a.left) / TK, hi = min(a.L - 1, min(b0 + RB, a.L) - 1 + a.right) / TK;
@@ -314,11 +314,11 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
     first = chunk;
     if (a.mask) {
       __syncthreads();  // the last chunk's words have been read
-      for (int t0 = 0; t0 < m; t0 += 16) {
+      for (int t0 = 0; t0 < m; t0 += 4 * W) {
         int mk[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int t = chunk + min(t0 + 4 * u + wave_id(), m - 1), r = (t < sink ? t : t + jump) * TK + lane;
+          const int t = chunk + min(t0 + W * u + wave_id(), m - 1), r = (t < sink ? t : t + jump) * TK + lane;
           const long at = (long)n * a.mask_n + min(r, a.L - 1);
           mk[u] = a.mask_bytes == 1 ? (int)reinterpret_cast<const unsigned char*>(a.mask)[at]
                                     : reinterpret_cast<const int*>(a.mask)[at];
@@ -327,7 +327,7 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const unsigned long long w = __ballot(mk[u] != 0);
-          const int t = t0 + 4 * u + wave_id();
+          const int t = t0 + W * u + wave_id();
           if (t < m && lane == 0) words[t] = w;
         }
       }
@@ -364,17 +364,17 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
   operands_here();
   while (t0 >= 0 || t1 >= 0) {  // t0: the tile worked on; t1: the tile being read
     if (t1 >= 0) {
-      lk.issue(t1 * TK, a.L, buf ^ 1);
-      lv.issue(t1 * TK, a.L, buf ^ 1);
+      lk.issue(t1 * TK, a.L, (buf ^ 1) % B);
+      lv.issue(t1 * TK, a.L, (buf ^ 1) % B);
     }
-    if (t0 >= 0) each(kt[buf], vt[buf], t0 * TK, keep);
+    if (t0 >= 0) each(kt[buf % B], vt[buf % B], t0 * TK, keep);
     t0 = t1;
     keep = keep1;
     if (t1 >= 0) {
       landed();
       __syncthreads();
       buf ^= 1;
-      if (a.mask && keep != ~0ull) clear_rows<D>(kt[buf], vt[buf], keep);
+      if (a.mask && keep != ~0ull) clear_rows<D, W>(kt[buf % B], vt[buf % B], keep);
       t1 = next(keep1);
     }
   }
@@ -387,10 +387,10 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
 // rescaling of accumulators in nearly all blocks); all 2048 x 2048 pairs 500 - 590 us (820 - 700); 16 heads x 128,
 // 4 x 4096 causal, window 1024: 195 - 216 (600).  Workgroups of 8 waves read the keys half as often and took 229
 // against 187 us; 64 queries per wave 242 against 181 (registers).
-template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) unsigned short kt[2][TK * D];
-  __shared__ __attribute__((aligned(1024))) unsigned short vt[2][TK * D];
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short kt[W / 2][TK * D];
+  __shared__ __attribute__((aligned(1024))) unsigned short vt[W / 2][TK * D];
   __shared__ unsigned long long words[128];
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
   Frags<D> fr;
   fr.init();
   const Sees sees(a, w0);
-  walk_keys<D>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
+  walk_keys<D, W>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const unsigned kw = (unsigned)(keep >> (32 * c));
@@ -475,10 +475,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
 // do * o and goes to memory for the other kernel; -D is the start value of the dP accumulators (from zero,
 // subtracted later: 623 instead of 618 us, forward and backward of the forward's pages).  Those pages:
 // 229 - 267 us; four waves per SIMD spill and cost 35 us.
-template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) unsigned short kt[2][TK * D];
-  __shared__ __attribute__((aligned(1024))) unsigned short vt[2][TK * D];
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short kt[W / 2][TK * D];
+  __shared__ __attribute__((aligned(1024))) unsigned short vt[W / 2][TK * D];
   __shared__ unsigned long long words[128];
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const Where wg(blockIdx.x, gridDim.x / a.tiles, a.tiles);
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
   Frags<D> fr;
   fr.init();
   const Sees sees(a, w0);
-  walk_keys<D>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
+  walk_keys<D, W>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const unsigned kw = (unsigned)(keep >> (32 * c));
@@ -638,17 +638,17 @@ __device__ __forceinline__ bool key_lane(const Args& a, int n, int kvh, int j, K
   return ok;
 }
 
-template <int D>
-__global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) unsigned short tiles[4][TK * D];  // Q, Q, dO, dO
-  __shared__ __attribute__((aligned(16))) float ls[2][TK], ds[2][TK];
-  unsigned short(*const qt)[TK * D] = tiles, (*const gt)[TK * D] = tiles + 2;
+template <int D, int W, int B>
+__global__ __launch_bounds__(64 * W, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) unsigned short tiles[2 * B][TK * D];  // Q .., dO ..
+  __shared__ __attribute__((aligned(16))) float ls[B][TK], ds[B][TK];
+  unsigned short(*const qt)[TK * D] = tiles, (*const gt)[TK * D] = tiles + B;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int Hkv = a.H / a.G;
   const Where wg(blockIdx.x, gridDim.x / (a.tiles + a.far_wgs), a.tiles + a.far_wgs);
   const int kvh = wg.nh % Hkv, n = wg.nh / Hkv;
   // far: (head of the group, chunk of query tiles, 32-key block of sinks)
-  const bool far = wg.tile >= a.tiles;
+  const bool far = W == 4 && wg.tile >= a.tiles;
   const int x = wg.tile - a.tiles, gc = far ? x / a.far_blocks : 0, g0 = far ? gc / a.far_chunks : 0;
   const int b0 = far ? 0 : wg.tile * RB, w0 = far ? x % a.far_blocks * 32 : b0 + wave_id() * 32, j = w0 + (lane & 31);
   const float sl = a.scale * LOG2E;
@@ -670,7 +670,7 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
   const int my_last = min(a.L - 1, j < a.sinks ? a.L - 1 : j + a.left);
   Frags<D> fr;
   fr.init();
-  Loader<D> lq, lg;
+  Loader<D, W> lq, lg;
   lq.init(a.q.p + n * a.q.n + (long)(kvh * a.G + g0) * a.q.h, a.q.l, qt[0]);
   lg.init(a.go.p + n * a.go.n + (long)(kvh * a.G + g0) * a.go.h, a.go.l, gt[0]);
   const float *rl = a.lse + ((long)n * a.H + kvh * a.G + g0) * a.L, *rd = a.dd + ((long)n * a.H + kvh * a.G + g0) * a.L;
@@ -682,10 +682,10 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
     const bool more = it + 1 < total;
     const int r1 = (lo + t1) * TK;
     if (more) {
-      lq.issue(r1, a.L, buf ^ 1);
-      lg.issue(r1, a.L, buf ^ 1);
-      if (wave_id() == 0) floats_to_lds(rl, r1, a.L, ls_at + (buf ^ 1) * TK * 4);
-      if (wave_id() == 1) floats_to_lds(rd, r1, a.L, ds_at + (buf ^ 1) * TK * 4);
+      lq.issue(r1, a.L, (buf ^ 1) % B);
+      lg.issue(r1, a.L, (buf ^ 1) % B);
+      if (wave_id() == 0) floats_to_lds(rl, r1, a.L, ls_at + (buf ^ 1) % B * TK * 4);
+      if (wave_id() == 1) floats_to_lds(rd, r1, a.L, ds_at + (buf ^ 1) % B * TK * 4);
     }
     if (it >= 0) {
 #pragma unroll
@@ -695,7 +695,7 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
         const bool full = i0 >= full_lo && i0 <= full_hi;
         unsigned see = 0u;
         if (!full) see = ok ? bits_between(j - a.right - i0, my_last - i0) : 0u;
-        w.block(fr, qt[buf], gt[buf], 32 * c, &ls[buf][32 * c], &ds[buf][32 * c], sl, see, full);
+        w.block(fr, qt[buf % B], gt[buf % B], 32 * c, &ls[buf % B][32 * c], &ds[buf % B][32 * c], sl, see, full);
       }
     }
     if (more) {
@@ -712,11 +712,11 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a) {
       }
     }
   }
-  if (far) {  // the four waves' sums, added in wave order; wave wv finishes accumulator quad wv
+  if (W == 4 && far) {  // the four waves' sums, added in wave order; wave wv finishes accumulator quad wv
     const int wv = wave_id();
     const long slot = a.far_main + ((long)n * a.H + kvh * a.G + g0) * a.far_chunks + gc % a.far_chunks;
     float* red = reinterpret_cast<float*>(&tiles[0][0]);  // 4 x 1024 floats
-    static_assert(sizeof(tiles) >= 4 * 1024 * sizeof(float), "the waves' sums fit the tiles' place");
+    static_assert(W < 4 || sizeof(tiles) >= 4 * 1024 * sizeof(float), "the waves' sums fit the tiles' place");
     auto finish = [&](const f32x16& x, int which, int e) {
       __syncthreads();
 #pragma unroll
@@ -860,9 +860,16 @@ PV_API int pv_wattn_fwd(const void* q, const void* k, const void* v, void* o, co
   if (!lse != !rest) return -5;
   const Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, rest, L, H, G, left, right, sinks, scale);
   const dim3 grid((unsigned)((long)a.tiles * H * N));
-  if (d == 32) hipLaunchKernelGGL(fwd_kernel<32>, grid, dim3(NTH), 0, (hipStream_t)stream, a);
-  else if (d == 64) hipLaunchKernelGGL(fwd_kernel<64>, grid, dim3(NTH), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(fwd_kernel<128>, grid, dim3(NTH), 0, (hipStream_t)stream, a);
+  hipStream_t s = (hipStream_t)stream;
+#define PV_WFWD(DV)                                                                                   \
+  do {                                                                                                \
+    if (L <= SHORT) hipLaunchKernelGGL((fwd_kernel<DV, 2>), grid, dim3(128), 0, s, a);                \
+    else hipLaunchKernelGGL((fwd_kernel<DV, 4>), grid, dim3(256), 0, s, a);                           \
+  } while (0)
+  if (d == 32) PV_WFWD(32);
+  else if (d == 64) PV_WFWD(64);
+  else PV_WFWD(128);
+#undef PV_WFWD
   PV_LAUNCH_CHECK();
   return 0;
 }
@@ -896,12 +903,15 @@ PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void*
   a.far_wgs = f.wgs;
   const dim3 gq((unsigned)((long)a.tiles * H * N)), gk((unsigned)((long)(a.tiles + f.wgs) * (H / G) * N));
   hipStream_t s = (hipStream_t)stream;
-#define PV_WBWD(DV)                                                 \
-  do {                                                              \
-    hipLaunchKernelGGL(bwd_dq_kernel<DV>, gq, dim3(NTH), 0, s, a);  \
-    PV_LAUNCH_CHECK();                                              \
-    hipLaunchKernelGGL(bwd_dkv_kernel<DV>, gk, dim3(NTH), 0, s, a); \
-    PV_LAUNCH_CHECK();                                              \
+#define PV_WBWD(DV)                                                                                   \
+  do {                                                                                                \
+    if (L <= SHORT) hipLaunchKernelGGL((bwd_dq_kernel<DV, 2>), gq, dim3(128), 0, s, a);               \
+    else hipLaunchKernelGGL((bwd_dq_kernel<DV, 4>), gq, dim3(256), 0, s, a);                          \
+    PV_LAUNCH_CHECK();                                                                                \
+    if (L <= SHORT && G == 1) hipLaunchKernelGGL((bwd_dkv_kernel<DV, 2, 1>), gk, dim3(128), 0, s, a); \
+    else if (L <= SHORT) hipLaunchKernelGGL((bwd_dkv_kernel<DV, 2, 2>), gk, dim3(128), 0, s, a);      \
+    else hipLaunchKernelGGL((bwd_dkv_kernel<DV, 4, 2>), gk, dim3(256), 0, s, a);                      \
+    PV_LAUNCH_CHECK();                                                                                \
   } while (0)
   if (d == 32) PV_WBWD(32);
   else if (d == 64) PV_WBWD(64);
