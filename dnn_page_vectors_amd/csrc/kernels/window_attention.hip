@@ -306,12 +306,12 @@ struct Where {
 };
 
 // Walks the key tiles that queries b0 .. b0 + RB - 1 see (the tiles of the sinks, then the window's):
-// `each(tile K, tile V, first key, keep bits)`.  While a tile is worked on, the next one is on its way to the
+// `each(tile K, tile V, first key, keep bits)`; `meanwhile()` while the first one is on its way.  While a tile is worked on, the next one is on its way to the
 // other buffer.  The mask is read ahead for 128 tiles at once, as one word per tile in LDS: tiles without
 // a key that counts cost nothing (a page's padding is such a run of tiles).  B = 1: there is one tile only.
-template <int D, int W, int B, typename F>
+template <int D, int W, int B, typename S, typename F>
 __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0, unsigned short (&kt)[B][TK * D],
-                                          unsigned short (&vt)[B][TK * D], unsigned long long (&words)[128], F each) {
+                                          unsigned short (&vt)[B][TK * D], unsigned long long (&words)[128], S meanwhile, F each) {
   const int lane = threadIdx.x & 63;
   const unsigned short* K = a.k.p + n * a.k.n + kvh * a.k.h;
   const unsigned short* V = a.v.p + n * a.v.n + kvh * a.v.h;
@@ -374,24 +374,28 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
     }
     return tile;
   };
+  auto read = [&](int tile, int buf) {
+    lk.issue(tile * TK, a.L, buf % B);
+    lv.issue(tile * TK, a.L, buf % B);
+  };
   unsigned long long keep = 0ull, keep1;
-  int t0 = -1, t1 = next(keep1), buf = 1;
-  operands_here();
-  while (t0 >= 0 || t1 >= 0) {  // t0: the tile worked on; t1: the tile being read
-    if (t1 >= 0) {
-      lk.issue(t1 * TK, a.L, (buf ^ 1) % B);
-      lv.issue(t1 * TK, a.L, (buf ^ 1) % B);
-    }
-    if (t0 >= 0) each(kt[buf % B], vt[buf % B], t0 * TK, keep);
+  int t0, t1 = next(keep1), buf = 0;  // t0: the tile worked on; t1: the tile being read
+  const bool any = t1 >= 0;
+  if (any) read(t1, 0);
+  meanwhile();
+  operands_here();  // the first tile too
+  if (!any) return;
+  while (true) {
+    __syncthreads();
     t0 = t1;
     keep = keep1;
-    if (t1 >= 0) {
-      landed();
-      __syncthreads();
-      buf ^= 1;
-      if (a.mask && keep != ~0ull) clear_rows<D, W>(kt[buf % B], vt[buf % B], keep);
-      t1 = next(keep1);
-    }
+    if (a.mask && keep != ~0ull) clear_rows<D, W>(kt[buf % B], vt[buf % B], keep);
+    t1 = next(keep1);
+    if (t1 >= 0) read(t1, buf ^ 1);
+    each(kt[buf % B], vt[buf % B], t0 * TK, keep);
+    if (t1 < 0) return;
+    landed();
+    buf ^= 1;
   }
 }
 
@@ -421,7 +425,7 @@ __global__ __launch_bounds__(64 * W, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
   Frags<D> fr;
   fr.init();
   const Sees sees(a, w0);
-  walk_keys<D, W>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
+  walk_keys<D, W>(a, n, hd / a.G, b0, kt, vt, words, [] {}, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const unsigned kw = (unsigned)(keep >> (32 * c));
@@ -507,31 +511,33 @@ __global__ __launch_bounds__(64 * W, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a)
   bf16x8 qf[D / 16], gf[D / 16];
   glob_frag<D>(a.q.p + n * a.q.n + (long)ic * a.q.l + hd * a.q.h, i < a.L, qf);
   glob_frag<D>(a.go.p + n * a.go.n + (long)ic * a.go.l + hd * a.go.h, i < a.L, gf);
-  float dd = 0.f;
-  {
-    bf16x8 of[D / 16];
-    glob_frag<D>(a.o.p + n * a.o.n + (long)ic * a.o.l + hd * a.o.h, i < a.L, of);
+  bf16x8 of[D / 16];
+  glob_frag<D>(a.o.p + n * a.o.n + (long)ic * a.o.l + hd * a.o.h, i < a.L, of);
+  uint2 rest[D / 16];
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const uint2 rest = *reinterpret_cast<const uint2*>(rest_at<D>(a, n, hd, ic, 2 * s + h));
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        dd = fmaf(with_rest((unsigned short)of[s][e], (int)((e < 4 ? rest.x : rest.y) << (24 - 8 * (e & 3))) >> 24),
-                  bf16_to_f32((unsigned short)gf[s][e]), dd);
-    }
-  }
-  dd += other_half(dd, h);
+  for (int s = 0; s < D / 16; ++s) rest[s] = *reinterpret_cast<const uint2*>(rest_at<D>(a, n, hd, ic, 2 * s + h));
   const long row = ((long)n * a.H + hd) * a.L + ic;
   const float nlse = a.lse[row];
-  if (i < a.L && h == 0) a.dd[row] = -dd;
-  const f32x16 minus_d = splat16(-dd);
+  f32x16 minus_d;
+  auto row_sum = [&] {
+    float dd = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        dd = fmaf(with_rest((unsigned short)of[s][e], (int)((e < 4 ? rest[s].x : rest[s].y) << (24 - 8 * (e & 3))) >> 24),
+                  bf16_to_f32((unsigned short)gf[s][e]), dd);
+    dd += other_half(dd, h);
+    if (i < a.L && h == 0) a.dd[row] = -dd;
+    minus_d = splat16(-dd);
+  };
   f32x16 acc[D / 32];
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) acc[c] = splat16(0.f);
   Frags<D> fr;
   fr.init();
   const Sees sees(a, w0);
-  walk_keys<D, W>(a, n, hd / a.G, b0, kt, vt, words, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
+  walk_keys<D, W>(a, n, hd / a.G, b0, kt, vt, words, row_sum, [&](const unsigned short* k, const unsigned short* v, int j0, unsigned long long keep) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const unsigned kw = (unsigned)(keep >> (32 * c));
@@ -692,42 +698,37 @@ __global__ __launch_bounds__(64 * W, D <= 64 ? 3 : 1) void bwd_dkv_kernel(Args a
   lg.init(a.go.p + n * a.go.n + (long)(kvh * a.G + g0) * a.go.h, a.go.l, gt[0]);
   const float *rl = a.lse + ((long)n * a.H + kvh * a.G + g0) * a.L, *rd = a.dd + ((long)n * a.H + kvh * a.G + g0) * a.L;
   const unsigned ls_at = lds_at(ls[0]), ds_at = lds_at(ds[0]);
-  int t1 = 0;  // the tile being read, within its head
-  int buf = 1, i0t = 0;
-  operands_here();
-  for (int it = -1; it < total; ++it) {
-    const bool more = it + 1 < total;
+  int t1 = 0, i0t;  // the tile being read, within its head; the first query of the tile worked on
+  auto read = [&](int buf) {
     const int r1 = (lo + t1) * TK;
-    if (more) {
-      lq.issue(r1, a.L, (buf ^ 1) % B);
-      lg.issue(r1, a.L, (buf ^ 1) % B);
-      if (wave_id() == 0) floats_to_lds(rl, r1, a.L, ls_at + (buf ^ 1) % B * TK * 4);
-      if (wave_id() == 1) floats_to_lds(rd, r1, a.L, ds_at + (buf ^ 1) % B * TK * 4);
+    lq.issue(r1, a.L, buf % B);
+    lg.issue(r1, a.L, buf % B);
+    if (wave_id() == 0) floats_to_lds(rl, r1, a.L, ls_at + buf % B * TK * 4);
+    if (wave_id() == 1) floats_to_lds(rd, r1, a.L, ds_at + buf % B * TK * 4);
+  };
+  if (total) read(0);
+  operands_here();  // the first tile too
+  for (int it = 0, buf = 0; it < total; ++it, buf ^= 1) {
+    __syncthreads();
+    i0t = (lo + t1) * TK;
+    if (++t1 == per) {  // the group's next head
+      t1 = 0;
+      lq.base += a.q.h * 2;
+      lg.base += a.go.h * 2;
+      rl += a.L;
+      rd += a.L;
     }
-    if (it >= 0) {
+    if (it + 1 < total) read(buf ^ 1);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int i0 = i0t + 32 * c;
-        if (i0 < none_lo || i0 > none_hi || (far && 2 * (it & 1) + c != wave_id())) continue;
-        const bool full = i0 >= full_lo && i0 <= full_hi;
-        unsigned see = 0u;
-        if (!full) see = ok ? bits_between(j - a.right - i0, my_last - i0) : 0u;
-        w.block(fr, qt[buf % B], gt[buf % B], 32 * c, &ls[buf % B][32 * c], &ds[buf % B][32 * c], sl, see, full);
-      }
+    for (int c = 0; c < 2; ++c) {
+      const int i0 = i0t + 32 * c;
+      if (i0 < none_lo || i0 > none_hi || (far && 2 * (it & 1) + c != wave_id())) continue;
+      const bool full = i0 >= full_lo && i0 <= full_hi;
+      unsigned see = 0u;
+      if (!full) see = ok ? bits_between(j - a.right - i0, my_last - i0) : 0u;
+      w.block(fr, qt[buf % B], gt[buf % B], 32 * c, &ls[buf % B][32 * c], &ds[buf % B][32 * c], sl, see, full);
     }
-    if (more) {
-      landed();
-      __syncthreads();
-      buf ^= 1;
-      i0t = r1;
-      if (++t1 == per) {  // the group's next head
-        t1 = 0;
-        lq.base += a.q.h * 2;
-        lg.base += a.go.h * 2;
-        rl += a.L;
-        rd += a.L;
-      }
-    }
+    landed();
   }
   if (W == 4 && far) {  // the four waves' sums, added in wave order; wave wv finishes accumulator quad wv
     const int wv = wave_id();
