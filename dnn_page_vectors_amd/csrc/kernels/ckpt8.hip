@@ -17,11 +17,9 @@
 // A thread takes 8 consecutive columns of a row (16-byte accesses of bf16, 8-byte of q) and four
 // neighbours share a block's maximum by two lane exchanges.  The accesses are declared with their element's
 // alignment, so rows of any length take them (global memory is read and written at any address).  The piece
-// that a row ends in (ODD: rows that are no multiple of 8, kernels of their own for their registers: with the tail
-// code in, 73728 x 2048 bias + GELU took 328 us instead of 317) reads on into the next row and is stored by
-// elements; only in the last rows it is read by elements too.
-#include <type_traits>
-
+// that a row ends in (ODD: rows that are no multiple of 8, kernels of their own: with this code in, 73728 x 2048
+// bias + GELU took 328 us instead of 317) reads the row's last 8 columns and shifts its own down; it is stored by
+// elements.  Rows of fewer than 8 columns are read by elements too.
 #include "common.h"
 
 namespace pv {
@@ -53,13 +51,9 @@ __device__ __forceinline__ float load1(const unsigned short* p) { return bf16_to
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(unsigned short* p, float v) { *p = f32_to_bf16(v); }
 
-// 8 consecutive values; TAIL: n of them (n >= 8: all), zeros behind
-template <bool TAIL, typename T>
-__device__ __forceinline__ void load8(const T* p, int n, float (&x)[8]) {
-  if (TAIL && n < 8) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < n ? load1(p + i) : 0.f;
-  } else if constexpr (sizeof(T) == 4) {
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
     const f32x4_a4 a = reinterpret_cast<const f32x4_a4*>(p)[0], b = *reinterpret_cast<const f32x4_a4*>(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
@@ -70,6 +64,23 @@ __device__ __forceinline__ void load8(const T* p, int n, float (&x)[8]) {
       x[2 * i] = __uint_as_float(a[i] << 16);
       x[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
     }
+  }
+}
+// columns c .. of a row of D, of which n count (n >= 8: all); what lies behind them is zero
+template <bool ODD, typename T>
+__device__ __forceinline__ void load_cols(const T* row, int c, int D, int n, float (&x)[8]) {
+  if (!ODD) {
+    load8(row + c, x);
+  } else if (D < 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? load1(row + i) : 0.f;
+  } else {
+    const int by = max(0, 8 - n);
+    load8(row + c - by, x);
+#pragma unroll
+    for (int s = 4; s; s >>= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = by & s ? (i + s < 8 ? x[i + s] : 0.f) : x[i];
   }
 }
 template <typename T>
@@ -86,17 +97,19 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&x)[8]) {
         u32x4_a2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
   }
 }
-template <bool TAIL>
-__device__ __forceinline__ u32x2 load_bytes(const unsigned char* p, int n) {
-  if (!TAIL || n >= 8) {
-    const u32x2_a1 w = *reinterpret_cast<const u32x2_a1*>(p);
-    return u32x2{w[0], w[1]};
-  }
-  u32x2 w{0u, 0u};
+template <bool ODD>
+__device__ __forceinline__ u32x2 load_bytes(const unsigned char* row, int c, int D, int n) {
+  if (ODD && D < 8) {
+    u32x2 w{0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 7; ++i)
-    if (i < n) w[i / 4] |= (unsigned)p[i] << (8 * (i % 4));
-  return w;
+    for (int i = 0; i < 7; ++i)
+      if (i < n) w[i / 4] |= (unsigned)row[i] << (8 * (i % 4));
+    return w;
+  }
+  const int by = ODD ? max(0, 8 - n) : 0;
+  const u32x2_a1 v = *reinterpret_cast<const u32x2_a1*>(row + c - by);
+  const unsigned long long w = (((unsigned long long)v[1] << 32) | v[0]) >> (8 * by);
+  return u32x2{(unsigned)w, (unsigned)(w >> 32)};
 }
 __device__ __forceinline__ void store_bytes(unsigned char* p, int n, u32x2 w) {
   if (n >= 8) {
@@ -169,16 +182,6 @@ __device__ __forceinline__ Place place(const Shape& s) {
   p.on = p.sub < p.step && p.c < s.D;
   return p;
 }
-// body(first row, TAIL) over the workgroup's rows, U passes at a time; TAIL where a row's last piece may read behind
-// the last row of all (8 columns are at most 8 rows)
-template <int U, bool ODD, typename F>
-__device__ __forceinline__ void each_rows(const Shape& s, const Place& p, F body) {
-  for (long r = p.r0; r < p.r1; r += U * p.step) {
-    if (ODD && r - p.sub + U * p.step + 8 >= s.T) body(r, std::true_type());
-    else body(r, std::false_type());
-  }
-}
-
 // Bound by memory: 256000 x 768 bf16 in 134 us (4.4 TB/s), with bias and GELU 73728 x 2048 in 148 (5.1 TB/s); a
 // column per lane instead of 8 took 348 against 114 us at 73728 x 2047.  Slabs of columns that leave fewer threads
 // idle than whole rows do (96 of 256 are, at 768) were no faster: 202 -> 218 us with GELU.
@@ -193,12 +196,12 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) bias[i] = p.on && i < p.n ? b[p.c + i] : 0.f;
   }
-  each_rows<U, ODD>(s, p, [&](long r, auto tail) {  // lanes that share a block leave together: same sub
+  for (long r = p.r0; r < p.r1; r += U * p.step) {  // lanes that share a block leave together: same sub
     float v[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long rr = min(r + u * p.step, p.r1 - 1);
-      if (p.on) load8<tail>(x + rr * s.D + p.c, p.n, v[u]);
+      if (p.on) load_cols<ODD>(x + rr * s.D, p.c, s.D, p.n, v[u]);
       else
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
@@ -210,8 +213,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, cons
       unsigned m = 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if constexpr (MODE == 1) v[u][i] += bias[i];
-        v[u][i] = i < p.n ? v[u][i] : 0.f;  // what lies behind the row
+        if constexpr (MODE == 1) v[u][i] += bias[i];  // zero behind the row
         m = max(m, mag(v[u][i]));
       }
       m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, cons
         store8(y + rr * s.D + p.c, p.n, o);
       }
     }
-  });
+  }
 }
 
 // 256000 x 768 into bf16: 104 us (5.7 TB/s)
@@ -236,13 +238,13 @@ __global__ __launch_bounds__(256) void unpack_kernel(const unsigned char* __rest
                                                      const unsigned char* __restrict__ sc, T* __restrict__ x, Shape s) {
   const Place p = place<ODD>(s);
   if (!p.on) return;
-  each_rows<U, ODD>(s, p, [&](long r, auto tail) {
+  for (long r = p.r0; r < p.r1; r += U * p.step) {
     u32x2 w[U];
     int e[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long rr = min(r + u * p.step, p.r1 - 1);
-      w[u] = load_bytes<tail>(q + rr * s.D + p.c, p.n);
+      w[u] = load_bytes<ODD>(q + rr * s.D, p.c, s.D, p.n);
       e[u] = sc[rr * s.nb + p.c / BLK];
     }
 #pragma unroll
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(const unsigned char* __rest
       dequant8(w[u], e[u], v);
       store8(x + rr * s.D + p.c, p.n, v);
     }
-  });
+  }
 }
 
 // Bound by memory: 73728 x 2048 in 167 us (4.5 TB/s), column sums in the same pass, 5 us for their partial rows.
@@ -271,15 +273,15 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const unsigned char* __re
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
   if (p.on)
-    each_rows<U, ODD>(s, p, [&](long r, auto tail) {
+    for (long r = p.r0; r < p.r1; r += U * p.step) {
       u32x2 w[U];
       float gv[U][8];
       int e[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long rr = min(r + u * p.step, p.r1 - 1);
-        w[u] = load_bytes<tail>(q + rr * s.D + p.c, p.n);
-        load8<tail>(dy + rr * s.D + p.c, p.n, gv[u]);
+        w[u] = load_bytes<ODD>(q + rr * s.D, p.c, s.D, p.n);
+        load_cols<ODD>(dy + rr * s.D, p.c, s.D, p.n, gv[u]);
         e[u] = sc[rr * s.nb + p.c / BLK];
       }
 #pragma unroll
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const unsigned char* __re
         store8(dx + rr * s.D + p.c, p.n, d);
         if constexpr (Y) store8(yh + rr * s.D + p.c, p.n, o);
       }
-    });
+    }
   // rows of the workgroup's passes: sub 0 adds the others in order
 #pragma unroll
   for (int i = 0; i < 8; ++i) sh[threadIdx.x * 8 + i] = acc[i];

@@ -19,10 +19,11 @@
 namespace pv {
 namespace temb {
 
-// Up to here one launch, which compares every token with all others: at 2048 tokens 10 / 12 / 27 / 28 us where sorting
-// takes 31 / 30 / 42 / 48 (tables of 5000 x 64, 1024 x 300, 30522 x 768, 60000 x 512, Zipf ids).  Ids that are spread like this
-// meet between 3000 and 8000 tokens, but 2048 tokens of a single id are 87 against 28 us, and twice as many 173.
-constexpr int SMALL_T = 2048;
+// Up to here one launch, which compares every token with all others: at 4096 tokens 18 / 23 / 48 / 42 us where sorting
+// takes 31 / 31 / 43 / 50 (tables of 5000 x 64, 1024 x 300, 30522 x 768, 60000 x 512, Zipf ids), at 8192 30 / 45 / 94 / 75
+// against 33 / 32 / 48 / 53; the sort's five further launches cost another 15 us of host time.  The worst ids, all
+// the same: 173 against 29 us at 4096 tokens.
+constexpr int SMALL_T = 4096;
 constexpr int CHUNK = 32;  // sorted tokens per wave
 constexpr int ZROWS = 64;  // table rows per zeroing workgroup of the small path
 

@@ -129,7 +129,19 @@ def test_wide_rows(E, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [1500, 2049, 9000, 33 * 64])
+@pytest.mark.parametrize("V", [1, 2, 64, 65, 255, 256, 65534, 65535, 65536, 70000])
+def test_tables_of_sorted_tokens(V):
+    check(zipf(4500, V, V), V, 24, torch.float32, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [4095, 4096, 4097, 4128, 4129, 5121])
+def test_sizes_around_the_sort(T):
+    check(zipf(T, 700, T), 700, 36, torch.bfloat16, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1500, 2049, 9000, 33 * 64, 4097, 65 * 64])
 @pytest.mark.parametrize("kind", ["one id", "all padding", "two ids", "runs of 32", "runs of 64", "sorted down", "one late"])
 def test_runs(T, kind):
     """Runs that end on, begin on and span the borders of the sorted chunks."""
