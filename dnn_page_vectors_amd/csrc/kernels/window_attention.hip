@@ -402,9 +402,9 @@ __device__ __forceinline__ void walk_keys(const Args& a, int n, int kvh, int b0,
 // ------------------------------------------------------------------------------------ forward
 // Workgroup = 128 queries of one head; a wave owns 32 of them (lane & 31), both half-waves hold the
 // same queries and split the keys of each block.  Bound by instruction issue, vector and matrix about equally:
-// 12 heads x 64, 32 ragged pages x 2000 tokens, window 256 + 256: 173 - 187 us (about 400 TFLOP/s of visible pairs, no
+// 12 heads x 64, 32 ragged pages x 2000 tokens, window 256 + 256: 178 us (400 TFLOP/s of visible pairs, no
 // rescaling of accumulators in nearly all blocks); all 2048 x 2048 pairs 500 - 590 us (820 - 700); 16 heads x 128,
-// 4 x 4096 causal, window 1024: 195 - 216 (600).  Workgroups of 8 waves read the keys half as often and took 229
+// 4 x 4096 causal, window 1024: 197 (610).  Workgroups of 8 waves read the keys half as often and took 229
 // against 187 us; 64 queries per wave 242 against 181 (registers).
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(64 * W, D <= 64 ? 4 : 2) void fwd_kernel(Args a) {
 // Same walk as the forward: dS^T in registers, dq^T += K^T dS^T.  D is the lane's own row sum of
 // do * o and goes to memory for the other kernel; -D is the start value of the dP accumulators (from zero,
 // subtracted later: 623 instead of 618 us, forward and backward of the forward's pages).  Those pages:
-// 229 - 267 us; four waves per SIMD spill and cost 35 us.
+// 228 us; four waves per SIMD spill and cost 35 us.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) unsigned short kt[W / 2][TK * D];
@@ -576,8 +576,8 @@ __global__ __launch_bounds__(64 * W, D <= 64 ? 3 : 2) void bwd_dq_kernel(Args a)
 // ------------------------------------------------------------------------------------ backward: dk, dv
 // Workgroup = 128 keys of one key/value head, a wave owns 32 of them; it walks the query tiles of
 // every query head of the group: P and dS (queries x keys), dv^T += dO^T P, dk^T += Q^T dS.  The rows'
-// -D are the start values of the dP accumulators, read from LDS into place.  The forward's pages: 296 - 303 us with
-// the far queries; heads of 128: one wave per SIMD (321 registers), 426 - 446 us, and a tile's two blocks taken
+// -D are the start values of the dP accumulators, read from LDS into place.  The forward's pages: 269 us with
+// the far queries; heads of 128: one wave per SIMD (321 registers), 414 us, and a tile's two blocks taken
 // together, products under exponentials, need more than 512 (spills: 741 -> 976 us, forward and backward).
 //
 // The sinks are seen by every later query: walked by their own workgroup alone they would make it the last
