@@ -232,6 +232,30 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, cons
   }
 }
 
+// y = gelu(x + b) where nothing is kept, in pack_kernel's arithmetic.  A workgroup takes a slab of 1024 columns of `rows`
+// rows, slabs of a row in neighbouring workgroups.  Bound by memory: 73728 x 2048 in 117 us (5.2 TB/s), 256000 x 768 in 152;
+// as a form of pack_kernel that stores no checkpoint 124 and 158.
+template <bool ODD>
+__global__ __launch_bounds__(128) void gelu_kernel(const unsigned short* __restrict__ x, const float* __restrict__ b,
+                                                   unsigned short* __restrict__ y, long T, int D, int slabs, int rows) {
+  const int c = (int)(blockIdx.x % slabs) * 1024 + threadIdx.x * 8, n = ODD ? D - c : 8;
+  if (c >= D) return;
+  float bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bias[i] = i < n ? b[c + i] : 0.f;
+  const long r0 = (long)(blockIdx.x / slabs) * rows, r1 = min(T, r0 + rows);
+  for (long r = r0; r < r1; ++r) {
+    float v[8];
+    load_cols<ODD>(x + r * D, c, D, n, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] += bias[i];
+      v[i] *= sig(v[i]);
+    }
+    store8(y + r * D + c, n, v);
+  }
+}
+
 // 256000 x 768 into bf16: 104 us (5.7 TB/s)
 template <typename T, int U, bool ODD>
 __global__ __launch_bounds__(256) void unpack_kernel(const unsigned char* __restrict__ q,
@@ -402,11 +426,20 @@ PV_API int pv_ckpt8_unpack(const void* q, const void* s, void* x, int x16, long 
   return x16 ? unpack(qq, ss, (unsigned short*)x, T, D, st) : unpack(qq, ss, (float*)x, T, D, st);
 }
 
-// x (T, D) bf16, b (D) fp32 -> y = gelu(x + b) bf16 and the checkpoint of x + b
+// x (T, D) bf16, b (D) fp32 -> y = gelu(x + b) bf16 and the checkpoint of x + b (q and s both null: y alone)
 PV_API int pv_ckpt8_gelu_fwd(const void* x, const float* b, void* y, void* q, void* s, long T, int D, void* stream) {
   if (const int rc = sizes(T, D)) return rc;
-  return pack<unsigned short, 1>((const unsigned short*)x, b, (unsigned short*)y, (unsigned char*)q, (unsigned char*)s, T,
-                                 D, (hipStream_t)stream);
+  if (!q != !s) return -3;
+  hipStream_t st = (hipStream_t)stream;
+  if (q) return pack<unsigned short, 1>((const unsigned short*)x, b, (unsigned short*)y, (unsigned char*)q, (unsigned char*)s, T, D, st);
+  if (T == 0) return 0;
+  // 16 rows per workgroup; more where there are so many that the grid would pass 2^32 threads
+  const int slabs = (D + 1023) / 1024, rows = (int)max(16L, (T * slabs + (1L << 24) - 1) >> 24);
+  const dim3 grid((unsigned)((T + rows - 1) / rows * slabs));
+  if (D % 8) hipLaunchKernelGGL((gelu_kernel<true>), grid, dim3(128), 0, st, (const unsigned short*)x, b, (unsigned short*)y, T, D, slabs, rows);
+  else hipLaunchKernelGGL((gelu_kernel<false>), grid, dim3(128), 0, st, (const unsigned short*)x, b, (unsigned short*)y, T, D, slabs, rows);
+  PV_LAUNCH_CHECK();
+  return 0;
 }
 
 // floats of workspace of pv_ckpt8_gelu_bwd

@@ -194,11 +194,33 @@ class _BiasGelu8Fn(torch.autograd.Function):
         return dx, db.to(b.dtype)
 
 
+class _GeluAloneFn(torch.autograd.Function):
+    """y = gelu(x + b) on the GPU where nothing is kept, in the arithmetic of the differentiable form.  An autograd
+    function although it has no backward: torch refuses to lose a forward-mode tangent in it."""
+
+    @staticmethod
+    def forward(ctx, x, b):
+        x, b = x.contiguous(), b.float().contiguous()
+        y = torch.empty_like(x)
+        D = x.shape[-1]
+        with on_device(x):
+            check(lib().pv_ckpt8_gelu_fwd(P(x), P(b), P(y), None, None, x.numel() // D, D, stream(x.device)),
+                  "pv_ckpt8_gelu_fwd")
+        return y
+
+
+def _gelu_alone(x: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """gelu(x + b) where no gradient is wanted: the bits of the differentiable form, for the same widths and biases."""
+    if use_hip(x):
+        return _GeluAloneFn.apply(x, b)
+    return _gelu(x.contiguous().float() + b.float()).to(x.dtype)
+
+
 def bias_gelu(x: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """gelu(x + b), keeping x + b in 8 bits for the backward (transformer.py::bias_gelu keeps x in bf16)."""
     _bias_ok(x, b, "ckpt8.bias_gelu")
     if not (torch.is_grad_enabled() and (x.requires_grad or b.requires_grad)):
-        return tops.bias_gelu(x, b)  # nothing to keep
+        return _gelu_alone(x, b)
     if use_hip(x) and grad_sink.flat_of(b) is None:
         return _native.binding().bias_gelu8(x, b)
     return _BiasGelu8Fn.apply(x, b)
@@ -317,8 +339,8 @@ def ffn(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,
     _check_x(x, "ckpt8.ffn")
     if w1.dim() != 2 or w2.dim() != 2 or w1.shape[1] != x.shape[-1] or w2.shape[1] != w1.shape[0] or b1.shape != w1.shape[:1]:
         raise ValueError(f"ckpt8.ffn: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, b1 {tuple(b1.shape)}, w2 {tuple(w2.shape)} do not fit")
-    if not (torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad)):
-        return tops.ffn(x, w1, b1, w2, res=res)
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w1, b1, w2))):
+        return tops.linear(_gelu_alone(tops.linear(x, w1, res=res), b1), w2)
     if use_hip(x):
         return _FFN8Fn.apply(x, w1, b1, w2, tops.weight_bf16(w1), tops.weight_bf16(w2), res)
     return _RoundSaved.apply(bias_gelu(_RoundSaved.apply(x, w1), b1), w2)

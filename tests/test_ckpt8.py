@@ -404,3 +404,56 @@ def test_offsets_past_32_bits(D):
         del y
     for u, w in zip(*both):
         assert torch.equal(u, w)
+
+
+BIASES = {"fp32": lambda b: b, "bf16": lambda b: b.bfloat16(), "fp64": lambda b: b.double(),
+          "strided": lambda b: torch.stack([b, b - 9.0], 1)[:, 0]}
+
+
+def check_without_gradients(x, b):
+    """The result where nothing is kept is the differentiable form's, bit for bit, in its type."""
+    want = ckpt8.bias_gelu(x.detach().requires_grad_(), b)
+    for got in (ckpt8.bias_gelu(x, b), ckpt8.bias_gelu(x.t().contiguous().t(), b)):
+        assert got.dtype == want.dtype == x.dtype and got.shape == x.shape and torch.equal(got, want)
+    with torch.no_grad():
+        assert torch.equal(ckpt8.bias_gelu(x, b.detach().requires_grad_()), want)
+
+
+def check_ffn_without_gradients(x, w1, b1, w2):
+    want = ckpt8.ffn(x.detach().requires_grad_(), w1, b1, w2)
+    got = ckpt8.ffn(x, w1, b1, w2)
+    assert got.dtype == want.dtype and got.shape == want.shape and torch.equal(got, want)
+    c = b1.detach().requires_grad_()                     # the only operand with a gradient
+    (db,) = torch.autograd.grad(ckpt8.ffn(x, w1, c, w2).float().sum(), c)
+    assert db.dtype == c.dtype and db.shape == c.shape and bool(db.abs().sum() > 0) == (x.shape[0] > 0)
+
+
+def ffn_operands(T, I, D):
+    g = torch.Generator().manual_seed(I)
+    return (values(T, D, 8).float(), 0.2 * torch.randn(I, D, generator=g), torch.randn(I, generator=g),
+            0.2 * torch.randn(D, I, generator=g))
+
+
+@pytest.mark.parametrize("bias", BIASES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_cpu_without_gradients(bias, dtype):
+    b = BIASES[bias](torch.randn(33, generator=torch.Generator().manual_seed(1)))
+    check_without_gradients(values(5, 33, 4, dtype), b)
+    x, w1, b1, w2 = ffn_operands(5, 33, 40)
+    check_ffn_without_gradients(x, w1, BIASES[bias](b1), w2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", BIASES)
+@pytest.mark.parametrize("T,D", [(0, 40), (1, 1), (5, 7), (45, 300), (33, 2047), (33, 2048), (700, 2056)])
+def test_without_gradients(T, D, bias):
+    b = BIASES[bias](torch.randn(D, generator=torch.Generator().manual_seed(D)).cuda())
+    check_without_gradients(values(T, D, T).cuda(), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", BIASES)
+@pytest.mark.parametrize("T,I", [(0, 40), (3, 33), (70, 128)])
+def test_ffn_without_gradients(T, I, bias):
+    x, w1, b1, w2 = (t.cuda() for t in ffn_operands(T, I, 64))
+    check_ffn_without_gradients(x.bfloat16(), w1, BIASES[bias](b1), w2)
