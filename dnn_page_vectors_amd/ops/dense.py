@@ -94,12 +94,14 @@ def _colsum_ok(x: torch.Tensor, C: int, ldx: int) -> bool:
 
 
 def colsum(x: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False, scale=None, bias=None,
-           act: str = "none", scale_is_len: bool = False) -> torch.Tensor:
+           act: str = "none", scale_is_len: bool = False, ordered: bool = False) -> torch.Tensor:
     """Sum over the leading axis of x (R, ...) -> fp32 (...) on the HIP column-sum kernel
     (dense.hip::colsum_kernel): the bias gradients and split-K partial sums of the backward.
     ``accumulate``: add into ``out`` (a zeroed buffer or a flat-gradient region).
     ``scale`` (rows of the result) / ``bias`` (its last axis) / ``act``: fused epilogue
-    act(scale * sum + bias) of the split-K forward (no accumulate)."""
+    act(scale * sum + bias) of the split-K forward (no accumulate).
+    ``ordered``: every column by one workgroup, in an order that the sizes alone decide (no atomics;
+    no accumulate)."""
     R = x.shape[0]
     tail = x.shape[1:]
     C = 1
@@ -111,7 +113,7 @@ def colsum(x: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool
         E = int(tail[-1]) if len(tail) else 1
         if epi:
             mode = 3 if (scale_is_len and scale is not None) else 2
-        elif accumulate or R > 64:
+        elif accumulate or (R > 64 and not ordered):
             mode = 1
         else:
             mode = 0

@@ -415,17 +415,20 @@ class _BertEmbedFn(torch.autograd.Function):
 
 
 def _position_grads(g, groups, pos, typ, want_pos: bool, want_typ: bool):
-    """Position rows as per-group sums over the sequences of g (T, H), the type row as their total."""
+    """Position rows as per-group sums over the sequences of g (T, H), the type row as their total.  By the column-sum
+    kernel: torch's sum of many rows into few clears its counters by a memset, and in a captured step such a
+    memset left the type row's gradient wrong in every replay after the first."""
     H = g.shape[1]
     dpos = torch.zeros(pos.shape, dtype=torch.float32, device=g.device)
     dtyp = None
     off = 0
     for N, L in groups:
-        dpos[:L] += torch.sum(g[off:off + N * L].view(N, L, H), dim=0, dtype=torch.float32)
+        if N * L:
+            dpos[:L] += dops.colsum(g[off:off + N * L].view(N, L, H), ordered=True)
         off += N * L
     if want_typ:
         dtyp = torch.zeros(typ.shape, dtype=torch.float32, device=g.device)
-        dtyp[0] = dpos.sum(0)
+        dops.colsum(dpos, out=dtyp[0], ordered=True)
     return (dpos if want_pos else None), dtyp
 
 

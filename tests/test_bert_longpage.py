@@ -1,5 +1,7 @@
 """The long-page transformer tower: scaled lookup, windowed attention and 8-bit checkpoints run together, through the
 model, the trainer and encode()."""
+import ctypes
+
 import pytest
 import torch
 
@@ -181,3 +183,80 @@ def test_captured_step_replays():
                 continue                             # torch's own sums (see below)
             # bias and LayerNorm sums of the dense layers add by atomics: any order of T terms
             assert torch.allclose(x, y, rtol=1e-3, atol=1e-4 * float(y.abs().max()) + 1e-12), (rep, n)
+
+
+def node_kinds(graph):
+    """How many nodes of each kind a captured graph holds (0 kernel, 1 copy, 2 memset)."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    raw, n = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(raw, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert hip.hipGraphGetNodes(raw, nodes, ctypes.byref(n)) == 0
+    kinds = []
+    for x in nodes:
+        t = ctypes.c_int(-1)
+        assert hip.hipGraphNodeGetType(ctypes.c_void_p(x), ctypes.byref(t)) == 0
+        kinds.append(t.value)
+    return {k: kinds.count(k) for k in set(kinds)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(bert_window=0, bert_ckpt8=False, bert_embed_scale=0.0)])
+def test_captured_step_replays_position_and_type_gradients(kw):
+    """Tables of 2000 positions, whose sum into the type row torch would split over workgroups.  At 256 columns nothing
+    on the way to these gradients is added by atomics: the same bits in every replay as in the eager step."""
+    cfg = config(loss_mode="in_batch", bert_max_len=2000, document_length=300, bert_hidden=256, bert_heads=4, **kw)
+    dev = torch.device("cuda:0")
+    m = build_model(cfg, 400).to(dev)
+    m.train()
+    q, d = pair_batch(cfg, dev)
+    ps = list(m.parameters())
+
+    def step():
+        return torch.autograd.grad(loss_of(m, q, d), ps)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        got = step()
+    assert 2 not in node_kinds(graph)
+    for rep in range(4):
+        a, b = pair_batch(cfg, dev, seed=20 + rep)
+        q.copy_(a)
+        d.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for (n, _), x, y in zip(m.named_parameters(), got, step()):
+            if n.endswith((".pos", ".typ")):
+                assert y.abs().max() > 0 and torch.equal(x, y), (rep, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [[(1, 1)], [(3, 7), (5, 40)], [(200, 5), (0, 9), (2, 1999)], [(70, 33)]])
+def test_position_and_type_gradients(groups):
+    """Against 64 bits: a sum of n fp32 terms in any order is off by n 2^-24 of the sum of magnitudes."""
+    from dnn_page_vectors_amd.ops import transformer as tops
+
+    H, P = 96, 2000
+    T = sum(N * L for N, L in groups)
+    g = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).bfloat16()
+    want, mag, terms = torch.zeros(P, H).double(), torch.zeros(P, H).double(), 0
+    off = 0
+    for N, L in groups:
+        part = g[off:off + N * L].view(N, L, H).double()
+        want[:L] += part.sum(0)
+        mag[:L] += part.abs().sum(0)
+        terms += N
+        off += N * L
+    pos, typ = torch.zeros(P, H, device="cuda"), torch.zeros(2, H, device="cuda")
+    dpos, dtyp = tops._position_grads(g.cuda(), groups, pos, typ, True, True)
+    assert ((dpos.double().cpu() - want).abs() <= (terms + 1) * 2.0 ** -24 * mag).all()
+    assert ((dtyp[0].double().cpu() - want.sum(0)).abs() <= (terms + P + 1) * 2.0 ** -24 * mag.sum(0)).all()
+    assert not dtyp[1].any()
+    again = tops._position_grads(g.cuda(), groups, pos, typ, True, True)
+    assert torch.equal(dpos, again[0]) and torch.equal(dtyp, again[1])
