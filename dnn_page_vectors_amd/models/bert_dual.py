@@ -162,7 +162,7 @@ class BertEncoder(nn.Module):
         N, L = ids.shape
         mask = (ids != 0)
         mask[:, 0] = True  # [CLS] position always attends
-        x = (self._tokens(ids) + self.pos[:L].unsqueeze(0) + self.typ[0]).to(dt)
+        x = tops.add_positions(self._tokens(ids), self.pos, self.typ).to(dt)
         x = tops.add_layernorm(x, None, self.ln_g, self.ln_b)
         if training and p_drop > 0:
             x = F.dropout(x, p_drop, True)
@@ -192,8 +192,7 @@ class BertEncoder(nn.Module):
             for ids in ids_list:
                 ids = ids.long()
                 N, L = ids.shape
-                xs.append((self._tokens(ids) + self.pos[:L].unsqueeze(0) + self.typ[0]).to(dt)
-                          .reshape(N * L, -1))
+                xs.append(tops.add_positions(self._tokens(ids), self.pos, self.typ).to(dt).reshape(N * L, -1))
             x = torch.cat(xs, 0) if len(xs) > 1 else xs[0]
         x = tops.add_layernorm(x, None, self.ln_g, self.ln_b)
         if training and p_drop > 0:

@@ -432,6 +432,31 @@ def _position_grads(g, groups, pos, typ, want_pos: bool, want_typ: bool):
     return (dpos if want_pos else None), dtyp
 
 
+class _AddPositionsFn(torch.autograd.Function):
+    """tokens (N, L, H) fp32 + pos[l] + typ[0], the tables' gradients by _position_grads: autograd's own would be torch
+    sums, whose memsets a captured step cannot hold."""
+
+    @staticmethod
+    def forward(ctx, tokens, pos, typ):
+        ctx.params = (pos, typ)
+        return tokens + pos[:tokens.shape[1]].unsqueeze(0) + typ[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        pos, typ = ctx.params
+        N, L, H = g.shape
+        dpos, dtyp = _position_grads(g.reshape(N * L, H), [(N, L)], pos, typ, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return g, dpos, dtyp
+
+
+def add_positions(tokens: torch.Tensor, pos: torch.Tensor, typ: torch.Tensor) -> torch.Tensor:
+    """tokens (N, L, H) + pos[:L] + typ[0]."""
+    if use_hip(tokens):
+        return _AddPositionsFn.apply(tokens, pos, typ)
+    return tokens + pos[:tokens.shape[1]].unsqueeze(0) + typ[0]
+
+
 class _ScaledBertEmbedFn(torch.autograd.Function):
     """_BertEmbedFn with bf16(scale * word[id] + pos[l] + typ[0]) and the word-table gradient summed over the
     sorted tokens (csrc/kernels/token_embedding.hip): no atomics, so the deterministic mode takes it too.

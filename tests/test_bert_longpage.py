@@ -237,6 +237,13 @@ def test_captured_step_replays_position_and_type_gradients(kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(bert_window=0, bert_ckpt8=False, bert_embed_scale=0.0)])
+def test_captured_step_of_separate_towers(kw):
+    """The same where each tower runs alone, its position and type rows added to the token rows."""
+    test_captured_step_replays_position_and_type_gradients(dict(share_doc_tower=False, **kw))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("groups", [[(1, 1)], [(3, 7), (5, 40)], [(200, 5), (0, 9), (2, 1999)], [(70, 33)]])
 def test_position_and_type_gradients(groups):
     """Against 64 bits: a sum of n fp32 terms in any order is off by n 2^-24 of the sum of magnitudes."""
