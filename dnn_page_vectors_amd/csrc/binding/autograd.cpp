@@ -75,6 +75,11 @@ variable_list once(variable_list&& out, const char* what) {
   return (*err)(std::move(out));
 }
 
+// The kernels run below autograd, where a forward-mode tangent would be lost: an error, not a silent result without one.
+void refuse_tangents(std::initializer_list<const Tensor*> ts, const char* what) {
+  for (const Tensor* t : ts) TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -172,6 +177,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
 
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask, int64_t left,
                         int64_t right, int64_t sinks, double scale) {
+  refuse_tangents({&q, &k, &v}, "window_attention");
   if (wants_grad({&q, &k, &v})) {
     check_capture({&q, &k, &v}, "window_attention");
     return WindowAttention::apply(q, k, v, mask, left, right, sinks, scale);
@@ -229,6 +235,7 @@ struct ScaledEmbedding : torch::autograd::Function<ScaledEmbedding> {
 };
 
 Tensor scaled_embedding(const Tensor& W, const Tensor& ids, double scale, int64_t pad, bool bf16) {
+  refuse_tangents({&W}, "scaled_embedding");
   if (wants_grad({&W})) {
     check_capture({&W}, "scaled_embedding");
     return ScaledEmbedding::apply(W, ids, scale, pad, bf16);
@@ -309,6 +316,7 @@ PYBIND11_MODULE(pagevec_torch, m) {
   m.def("pack", &pack, call_guard<gil_scoped_release>());
   m.def("unpack", &unpack, call_guard<gil_scoped_release>());
   m.def("bias_gelu8", [](const Tensor& x, const Tensor& b) {
+    refuse_tangents({&x, &b}, "ckpt8.bias_gelu");
     check_capture({&x, &b}, "ckpt8.bias_gelu");
     return Tensor(BiasGelu8::apply(x, b));
   }, call_guard<gil_scoped_release>());

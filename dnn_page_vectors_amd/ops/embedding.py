@@ -517,7 +517,8 @@ def scaled_embedding(ids: torch.Tensor, W: torch.Tensor, scale: float = 1.0, pad
 
     The gradient of W is summed in fp32 over the tokens sorted by id: one writer per row, the same
     bits on every run.  The row ``padding_idx`` gets no gradient.  On the GPU an id outside [0, V) gives
-    a row of NaN (which the trainer's non-finite guard sees) and adds to no gradient; the CPU raises."""
+    a row of NaN (which the trainer's non-finite guard sees) and adds to no gradient, where the
+    CPU raises; a forward-mode derivative is refused there."""
     if W.dim() != 2 or W.dtype not in (torch.float32, torch.bfloat16) and W.is_cuda or not W.is_floating_point():
         raise TypeError(f"scaled_embedding: W must be a 2-D float32 or bfloat16 table, got {W.dim()}-D {W.dtype}")
     if ids.dtype not in (torch.int32, torch.int64):

@@ -139,7 +139,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     head h // (H / Hkv)), mask (N, L) of the keys (non-zero = a real token; masked keys and values
     may hold anything) -> (N, L, H, d).  ``scale`` defaults to 1 / sqrt(d).
 
-    Differentiable once in q, k and v.  On the GPU: bf16, d in (32, 64, 128), any strides (operands
+    Differentiable once in q, k and v, on the GPU in reverse mode alone.  On the GPU: bf16, d in (32, 64, 128), any strides (operands
     whose rows are not 16-byte aligned are copied).  A non-finite value at a *visible* key may reach
     queries up to 64 tokens outside its window."""
     _check_qkv(q, k, v)

@@ -86,3 +86,45 @@ def test_two_threads_on_their_own_streams():
     for t in threads:
         t.join()
     assert not failed
+
+
+def forward_mode_calls(device):
+    """The operators as functions of operands that get tangents."""
+    from dnn_page_vectors_amd.ops import ckpt8
+    from dnn_page_vectors_amd.ops.embedding import scaled_embedding
+    from dnn_page_vectors_amd.ops.window_attention import packed_window_attention, window_attention
+
+    gen = torch.Generator().manual_seed(0)
+    mk = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(device)
+    q, x, b, w = mk(1, 8, 2, 32), mk(8, 32), mk(32).float(), mk(32, 32).float()
+    ids = torch.arange(4, device=device)
+    return {
+        "q": (lambda t: window_attention(t, q, q, 2, 2), q), "k": (lambda t: window_attention(q, t, q, 2, 2), q),
+        "v": (lambda t: window_attention(q, q, t, 2, 2), q),
+        "packed": (lambda t: packed_window_attention(t, [None], [(1, 8)], 2, 2, 2), mk(8, 192)),
+        "table": (lambda t: scaled_embedding(ids, t, 0.5), w),
+        "gelu": (lambda t: ckpt8.bias_gelu(t, b), x), "gelu bias": (lambda t: ckpt8.bias_gelu(x, t), b),
+        "linear": (lambda t: ckpt8.linear(t, w), x),
+        "ffn": (lambda t: ckpt8.ffn(t, w, b, w), x), "ffn bias": (lambda t: ckpt8.ffn(x, w, t, w), b),
+    }
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", ["q", "k", "v", "packed", "table", "gelu", "gelu bias", "linear", "ffn", "ffn bias"])
+def test_forward_mode_is_refused(name, grad):
+    """A tangent is never lost in silence: the kernels have no forward-mode form."""
+    f, t = forward_mode_calls("cuda")[name]
+    t = t.requires_grad_(grad)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            f(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        f(t)  # without a tangent the level does no harm
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "table", "gelu", "gelu bias", "ffn", "ffn bias"])
+def test_forward_mode_cpu(name):
+    f, t = forward_mode_calls("cpu")[name]
+    with torch.autograd.forward_ad.dual_level():
+        out = torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))))
+        assert out.tangent is not None and out.tangent.abs().max() > 0
