@@ -54,6 +54,22 @@ def _check_x(x: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: shape {tuple(x.shape)} is outside the kernels' range")
 
 
+def _check_packed(p: "Packed", name: str) -> None:
+    D = p.q.shape[-1] if p.q.dim() else 0
+    if D == 0:
+        raise ValueError(f"{name}: needs at least one column, got shape {tuple(p.q.shape)}")
+    if p.q.dtype != torch.uint8 or p.s.dtype != torch.uint8 or p.s.shape != (*p.q.shape[:-1], _blocks(D)):
+        raise ValueError(f"{name}: {tuple(p.q.shape)} {p.q.dtype} values do not go with {tuple(p.s.shape)} {p.s.dtype} scales")
+    if p.q.device != p.s.device:
+        raise ValueError(f"{name}: values and scales are on different devices")
+
+
+def _same_device(x: torch.Tensor, name: str, **others: Optional[torch.Tensor]) -> None:
+    for what, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: {what} is on {t.device}, x on {x.device}")
+
+
 def _pow2(e: torch.Tensor) -> torch.Tensor:
     """2^e (fp32), -126 <= e <= 127, from its bit pattern."""
     return ((e.int() + 127) << 23).view(torch.float32)
@@ -98,13 +114,7 @@ def unpack(p: Packed, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     dtype = p.dtype if dtype is None else dtype
     if dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"ckpt8.unpack: dtype must be bfloat16 or float32, got {dtype}")
-    D = p.q.shape[-1] if p.q.dim() else 0
-    if D == 0:
-        raise ValueError(f"ckpt8.unpack: needs at least one column, got shape {tuple(p.q.shape)}")
-    if p.q.dtype != torch.uint8 or p.s.dtype != torch.uint8 or p.s.shape != (*p.q.shape[:-1], _blocks(D)):
-        raise ValueError(f"ckpt8.unpack: {tuple(p.q.shape)} {p.q.dtype} values do not go with {tuple(p.s.shape)} {p.s.dtype} scales")
-    if p.q.device != p.s.device:
-        raise ValueError("ckpt8.unpack: values and scales are on different devices")
+    _check_packed(p, "ckpt8.unpack")
     if not use_hip(p.q):
         return _unpack_reference(p.q, p.s).to(dtype)
     return _native.binding().unpack(p.q, p.s, dtype == torch.bfloat16)
@@ -123,7 +133,10 @@ def _gelu_slope(u: torch.Tensor) -> torch.Tensor:
 
 
 def gelu_pack(x: torch.Tensor, b: torch.Tensor) -> Tuple[torch.Tensor, Packed]:
-    """y = gelu(x + b) and the checkpoint of x + b: x (..., D), b (D) fp32."""
+    """y = gelu(x + b) and the checkpoint of x + b: x (..., D) (bf16 on the GPU), b (D).  Not differentiable: what
+    bias_gelu and ffn are made of."""
+    _bias_ok(x, b, "ckpt8.gelu_pack")
+    x, b = x.detach().contiguous(), b.detach().float().contiguous()
     if not use_hip(x):
         u = x.float() + b.float()
         return _gelu(u).to(x.dtype), Packed(*_pack_reference(u), x.dtype)
@@ -137,16 +150,23 @@ def gelu_pack(x: torch.Tensor, b: torch.Tensor) -> Tuple[torch.Tensor, Packed]:
 
 
 def gelu_backward(p: Packed, dy: torch.Tensor, with_y: bool = False, db: Optional[torch.Tensor] = None):
-    """(dx, db, y): dx = dy gelu'(u) at the kept u, db (D) fp32 its column sums (added into ``db`` if given),
-    y = gelu(u) (``with_y``, else None)."""
+    """(dx, db, y): dx = dy gelu'(u) at the kept u, db (D) fp32 its column sums (added into ``db`` if given: contiguous
+    fp32), y = gelu(u) (``with_y``, else None)."""
+    _check_packed(p, "ckpt8.gelu_backward")
     D = p.q.shape[-1]
+    if dy.shape != p.q.shape or not dy.is_floating_point():
+        raise ValueError(f"ckpt8.gelu_backward: dy {tuple(dy.shape)} {dy.dtype} does not go with a checkpoint of {tuple(p.q.shape)}")
+    if db is not None and (db.shape != (D,) or db.dtype != torch.float32 or not db.is_contiguous()):
+        raise ValueError(f"ckpt8.gelu_backward: db must be {D} contiguous float32 sums, got {tuple(db.shape)} {db.dtype}")
+    _same_device(p.q, "ckpt8.gelu_backward", dy=dy, db=db)
     if not use_hip(dy):
         u = _unpack_reference(p.q, p.s)
         du = dy.float() * _gelu_slope(u)
         sums = du.reshape(-1, D).sum(0)
         sums = sums if db is None else db.add_(sums)
         return du.to(dy.dtype), sums, _gelu(u).to(p.dtype) if with_y else None
-    dy = dy.to(torch.bfloat16).contiguous()
+    q, s = p.q.contiguous(), p.s.contiguous()
+    dy = dy.detach().to(torch.bfloat16).contiguous()
     T = dy.numel() // D
     dx = torch.empty_like(dy)
     y = torch.empty_like(dy) if with_y else None
@@ -155,7 +175,7 @@ def gelu_backward(p: Packed, dy: torch.Tensor, with_y: bool = False, db: Optiona
         db = torch.empty(D, dtype=torch.float32, device=dy.device)
     with on_device(dy):
         ws = torch.empty(int(lib().pv_ckpt8_gelu_bwd_ws(T, D)), dtype=torch.float32, device=dy.device)
-        check(lib().pv_ckpt8_gelu_bwd(P(p.q), P(p.s), P(dy), P(dx), P(y), P(db), int(add), P(ws), T, D,
+        check(lib().pv_ckpt8_gelu_bwd(P(q), P(s), P(dy), P(dx), P(y), P(db), int(add), P(ws), T, D,
                                       stream(dy.device)), "pv_ckpt8_gelu_bwd")
     return dx, db, y
 
@@ -164,8 +184,7 @@ def _bias_ok(x: torch.Tensor, b: torch.Tensor, name: str) -> None:
     _check_x(x, name)
     if b.shape != (x.shape[-1],):
         raise ValueError(f"{name}: bias {tuple(b.shape)} does not go with {x.shape[-1]} columns")
-    if b.device != x.device:
-        raise ValueError(f"{name}: the bias is on {b.device}, x on {x.device}")
+    _same_device(x, name, bias=b)
     if use_hip(x) and x.dtype != torch.bfloat16:
         raise TypeError(f"{name}: the GPU kernels take bfloat16, got {x.dtype}")
 
@@ -293,6 +312,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None,
     _check_x(x, "ckpt8.linear")
     if w.dim() != 2 or w.shape[1] != x.shape[-1]:
         raise ValueError(f"ckpt8.linear: weight {tuple(w.shape)} does not go with {x.shape[-1]} columns")
+    if b is not None and b.shape != w.shape[:1]:
+        raise ValueError(f"ckpt8.linear: bias {tuple(b.shape)} does not go with {w.shape[0]} outputs")
+    _same_device(x, "ckpt8.linear", weight=w, bias=b)
     if not (torch.is_grad_enabled() and w.requires_grad):
         return tops.linear(x, w, b, res=res)
     if use_hip(x):
@@ -339,6 +361,7 @@ def ffn(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,
     _check_x(x, "ckpt8.ffn")
     if w1.dim() != 2 or w2.dim() != 2 or w1.shape[1] != x.shape[-1] or w2.shape[1] != w1.shape[0] or b1.shape != w1.shape[:1]:
         raise ValueError(f"ckpt8.ffn: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, b1 {tuple(b1.shape)}, w2 {tuple(w2.shape)} do not fit")
+    _same_device(x, "ckpt8.ffn", w1=w1, b1=b1, w2=w2)
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w1, b1, w2))):
         return tops.linear(_gelu_alone(tops.linear(x, w1, res=res), b1), w2)
     if use_hip(x):

@@ -457,3 +457,47 @@ def test_without_gradients(T, D, bias):
 def test_ffn_without_gradients(T, I, bias):
     x, w1, b1, w2 = (t.cuda() for t in ffn_operands(T, I, 64))
     check_ffn_without_gradients(x.bfloat16(), w1, BIASES[bias](b1), w2)
+
+
+def u8(*shape):
+    return torch.zeros(*shape, dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("call,err", [
+    (lambda: ckpt8.gelu_pack(torch.zeros(3, 4), torch.zeros(5)), ValueError),
+    (lambda: ckpt8.gelu_pack(torch.zeros(3, 4), torch.zeros(4, device="meta")), ValueError),
+    (lambda: ckpt8.gelu_pack(torch.zeros(3, 4, dtype=torch.int32), torch.zeros(4)), TypeError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 1), torch.bfloat16), torch.zeros(3, 40)), ValueError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 2), torch.bfloat16), torch.zeros(4, 40)), ValueError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 2), torch.bfloat16), torch.zeros(3, 40, device="meta")), ValueError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 2), torch.bfloat16), torch.zeros(3, 40, dtype=torch.int32)), ValueError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 2), torch.bfloat16), torch.zeros(3, 40), db=torch.zeros(39)), ValueError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 2), torch.bfloat16), torch.zeros(3, 40), db=torch.zeros(40).double()), ValueError),
+    (lambda: ckpt8.gelu_backward(ckpt8.Packed(u8(3, 40), u8(3, 2), torch.bfloat16), torch.zeros(3, 40), db=torch.zeros(80)[::2]), ValueError),
+    (lambda: ckpt8.linear(torch.zeros(3, 4), torch.zeros(2, 4), torch.zeros(3)), ValueError),
+    (lambda: ckpt8.linear(torch.zeros(3, 4), torch.zeros(2, 4), torch.zeros(2, device="meta")), ValueError),
+    (lambda: ckpt8.ffn(torch.zeros(3, 4), torch.zeros(8, 4), torch.zeros(8, device="meta"), torch.zeros(4, 8)), ValueError),
+])
+def test_refused_operands(call, err):
+    with pytest.raises(err):
+        call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [33, 64])
+def test_gelu_pack_and_backward_take_any_strides(D):
+    g = torch.Generator().manual_seed(D)
+    x, b, dy = values(20, D, 6).cuda(), torch.randn(D, generator=g).cuda(), torch.randn(20, D, generator=g).bfloat16().cuda()
+    turned = lambda t: t.t().contiguous().t()
+    y, p = ckpt8.gelu_pack(x, b)
+    for c in (torch.stack([b, b + 1], 1)[:, 0], b.double()):
+        y2, p2 = ckpt8.gelu_pack(turned(x), c)
+        assert torch.equal(y2, y) and torch.equal(p2.q, p.q) and torch.equal(p2.s, p.s)
+    want = ckpt8.gelu_backward(p, dy, with_y=True)
+    got = ckpt8.gelu_backward(ckpt8.Packed(turned(p.q), turned(p.s), p.dtype), turned(dy), with_y=True)
+    for u, v in zip(got, want):
+        assert torch.equal(u, v)
+    with pytest.raises(ValueError):
+        ckpt8.ffn(x[:, :32].contiguous(), torch.randn(64, 32).cuda(), torch.randn(64), torch.randn(32, 64).cuda())
+    with pytest.raises(TypeError):
+        ckpt8.gelu_pack(x.float(), b)
