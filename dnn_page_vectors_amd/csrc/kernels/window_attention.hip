@@ -805,13 +805,15 @@ __host__ inline View view(const void* p, const long* st, int i) {
   return View{(unsigned short*)const_cast<void*>(p), st[3 * i], st[3 * i + 1], st[3 * i + 2]};
 }
 
+// A launch holds fewer than 2^32 threads along an axis
+__host__ inline bool grid_holds(long workgroups, long L) { return workgroups * (L <= SHORT ? 128 : 256) < (1L << 32); }
+
 // sizes that the kernels' 32-bit row arithmetic and their 1-D grids hold
 __host__ inline int check_sizes(long N, long L, long H, long G, int d, float scale) {
   if (N <= 0 || L <= 0 || H <= 0 || G <= 0 || H % G) return -1;
   if (d != 32 && d != 64 && d != 128) return -2;
   if (L > (1L << 29) || !(scale > 0.f)) return -3;
-  const long blocks = (L + RB - 1) / RB * H * N;
-  return blocks > 0x7FFFFFFFL ? -4 : 0;
+  return grid_holds((L + RB - 1) / RB * H * N, L) ? 0 : -4;
 }
 
 // The far part of the sinks is split off where they all lie in the first workgroup of keys and it is long
@@ -831,7 +833,7 @@ __host__ inline FarPlan far_plan(long N, long L, long H, long G, int d, int left
   f.chunks = (int)((tiles - first + FAR - 1) / FAR);
   f.blocks = (sinks + 31) / 32;
   const long wgs = G * f.blocks * f.chunks;
-  if ((wgs + (L + RB - 1) / RB) * (H / G) * N > 0x7FFFFFFFL) return FarPlan{};
+  if (!grid_holds((wgs + (L + RB - 1) / RB) * (H / G) * N, L)) return FarPlan{};
   f.wgs = (int)wgs;
   f.near_slots = N * (H / G);
   f.floats = (f.near_slots + N * H * f.chunks) * 2 * d * sinks;

@@ -56,6 +56,14 @@ def _key_mask(mask: Optional[torch.Tensor], N: int, L: int, device) -> Optional[
     return mask if L == 1 or mask.stride(1) == 1 else mask.contiguous()
 
 
+def _check_range(N: int, L: int, H: int) -> None:
+    """A workgroup per 128 queries and head, of 128 threads for up to 64 tokens and 256 above, in a grid of fewer than
+    2^32 threads."""
+    if L > MAX_LEN or N * H * -(-L // 128) * (128 if L <= 64 else 256) >= 1 << 32:
+        raise ValueError(f"window_attention: {N} sequences of {L} tokens and {H} heads are outside the kernels' range "
+                         f"(length {MAX_LEN}, 2^25 heads of up to 64 tokens, 2^24 blocks of 128 queries of longer ones)")
+
+
 def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("window_attention: q, k, v must be (batch, length, heads, head dim)")
@@ -153,8 +161,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
         raise TypeError(f"window_attention: the GPU kernels take bfloat16, got {q.dtype}")
     if d not in HEAD_DIMS:
         raise ValueError(f"window_attention: head dim must be one of {HEAD_DIMS} on the GPU, got {d}")
-    if L > MAX_LEN or N * H * -(-L // 128) >= 1 << 31:
-        raise ValueError(f"window_attention: {tuple(q.shape)} is outside the kernels' range (length {MAX_LEN}, 2^31 blocks of 128 queries)")
+    _check_range(N, L, H)
     if q.numel() == 0:
         return q * 1.0
     return _native.binding().window_attention(q, k, v, mask, *win, scale)
@@ -223,6 +230,8 @@ def packed_window_attention(qkv: torch.Tensor, masks: Sequence[Optional[torch.Te
     masks = [_key_mask(m, N, L, qkv.device) for m, (N, L) in zip(masks, shapes)]
     if use_hip(qkv) and qkv.dtype == torch.bfloat16 and d in HEAD_DIMS and min((n for s in shapes for n in s), default=0) > 0 \
             and qkv.data_ptr() % 16 == 0 and qkv.shape[1] < 1 << 24:
+        for N, L in shapes:
+            _check_range(N, L, heads)
         train = torch.is_grad_enabled() and qkv.requires_grad
         if train:
             _native.binding().check_capture(qkv, "packed_window_attention")

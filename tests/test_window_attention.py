@@ -12,6 +12,7 @@ matrices.  One rounding to bf16 is off by at most h = 2^-8 relative.
 * dS = p (dP - D) is rounded once: its error E = p (err D + d 2^-23 |do||v|) + (h + e) |dS|;
   dq, dk: E against |k|, |q| and one rounding; dv: (h + e) P^T|do| and one rounding.
 """
+import ctypes
 import gc
 import math
 
@@ -510,3 +511,34 @@ def test_gpu_refusals():
     (ga,) = torch.autograd.grad(o, a, z, create_graph=True)
     with pytest.raises(RuntimeError):  # differentiable once
         torch.autograd.grad(ga.sum(), a)
+
+
+def test_shapes_beyond_the_grid_are_refused_by_every_layer():
+    """A launch holds fewer than 2^32 threads: 128 per head up to 64 tokens, 256 per 128 queries above."""
+    from dnn_page_vectors_amd import _native
+    from dnn_page_vectors_amd.ops.window_attention import _check_range
+
+    fwd = _native.hip(required=True).pv_wattn_fwd
+    for N, L, H in ((1 << 25, 1, 1), (1 << 22, 64, 8), (1 << 24, 65, 1), (1 << 20, 200, 8), (1, 1 << 29, 4)):
+        with pytest.raises(ValueError):
+            _check_range(N, L, H)
+        st = (ctypes.c_long * 12)()
+        assert fwd(None, None, None, None, st, None, 0, 1, None, None, N, L, H, 1, 32, 1, 1, 0, 0.5, None) == -4
+    for N, L, H in (((1 << 25) - 1, 1, 1), ((1 << 24) - 1, 65, 1), (1, 1 << 29, 3)):
+        _check_range(N, L, H)
+
+
+@pytest.mark.gpu
+def test_largest_grid_of_short_sequences():
+    """2^25 - 1 sequences of one token, the most that a launch holds; one more is refused."""
+    N, d = (1 << 25) - 1, 32
+    v = torch.randn(1, 1, 1, d, device="cuda").bfloat16()
+    one = torch.randn(1, 1, 1, d, device="cuda").bfloat16().expand(N, 1, 1, d)
+    out = window_attention(one, one, v.expand(N, 1, 1, d), 0, 0)
+    assert torch.equal(out[-3:], v.expand(3, 1, 1, d)) and bool((out == v).all())
+    more = one[:1].expand(N + 1, 1, 1, d)
+    with pytest.raises(ValueError):
+        window_attention(more, more, more, 0, 0)
+    packed = torch.zeros(1, 3 * d, device="cuda").bfloat16().expand(N + 1, 3 * d)
+    with pytest.raises(ValueError):
+        packed_window_attention(packed, [None], [(N + 1, 1)], 1, 0, 0)
