@@ -25,6 +25,7 @@ namespace temb {
 // the same: 173 against 29 us at 4096 tokens.
 constexpr int SMALL_T = 4096;
 constexpr int CHUNK = 32;  // sorted tokens per wave
+constexpr long MAX_T = 0x7FFFFFFFL - 4 * CHUNK;  // token numbers in 31 bits, and a grid of fewer than 2^32 threads for them
 constexpr int ZROWS = 64;  // table rows per zeroing workgroup of the small path
 
 struct Groups {
@@ -246,21 +247,23 @@ __global__ __launch_bounds__(256) void small_grad_kernel(Ids ids, const TG* __re
   }
   __shared__ int has[ZROWS];
   if (blockIdx.y) return;  // the zeroing workgroups take whole rows
-  const long r0 = (long)(blockIdx.x - T) * ZROWS;
-  if (threadIdx.x < ZROWS) has[threadIdx.x] = 0;
-  __syncthreads();
-  for (int u = threadIdx.x; u < T; u += 256) {
-    const long k = (long)ids.key(u, V, pad) - r0;
-    if (k >= 0 && k < ZROWS) has[k] = 1;
-  }
-  __syncthreads();
-  const int n = (int)min((long)ZROWS, V - r0);
-  for (int r = wave; r < n; r += 4) {
-    if (has[r]) continue;
-    float* row = dW + (r0 + r) * E;
-    const int whole = W == 4 ? E / 4 * 4 : 0;
-    for (int c = lane * 4; c < whole; c += 256) *reinterpret_cast<f32x4_a4*>(row + c) = f32x4_a4{0.f, 0.f, 0.f, 0.f};
-    for (int c = whole + lane; c < E; c += 64) row[c] = 0.f;
+  for (long r0 = (long)(blockIdx.x - T) * ZROWS; r0 < V; r0 += (long)(gridDim.x - T) * ZROWS) {
+    __syncthreads();
+    if (threadIdx.x < ZROWS) has[threadIdx.x] = 0;
+    __syncthreads();
+    for (int u = threadIdx.x; u < T; u += 256) {
+      const long k = (long)ids.key(u, V, pad) - r0;
+      if (k >= 0 && k < ZROWS) has[k] = 1;
+    }
+    __syncthreads();
+    const int n = (int)min((long)ZROWS, V - r0);
+    for (int r = wave; r < n; r += 4) {
+      if (has[r]) continue;
+      float* row = dW + (r0 + r) * E;
+      const int whole = W == 4 ? E / 4 * 4 : 0;
+      for (int c = lane * 4; c < whole; c += 256) *reinterpret_cast<f32x4_a4*>(row + c) = f32x4_a4{0.f, 0.f, 0.f, 0.f};
+      for (int c = whole + lane; c < E; c += 64) row[c] = 0.f;
+    }
   }
 }
 
@@ -503,6 +506,9 @@ __global__ __launch_bounds__(64 * JOIN) void join_kernel(const KT* __restrict__ 
   }
 }
 
+// workgroups of a launch: fewer than 2^32 threads along an axis
+__host__ inline long grid_limit(int threads) { return ((1L << 32) - 1) / threads; }
+
 __host__ inline size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct Layout {
@@ -574,8 +580,7 @@ int grad(const Ids& ids, const TG* g, float* dW, long T, long V, int E, long pad
          long ws_bytes, hipStream_t st) {
   if (T <= SMALL_T) {
     const int slabs = (E + 64 * W - 1) / (64 * W);
-    const long z = acc ? 0 : (V + ZROWS - 1) / ZROWS;
-    if (T + z > 0x7FFFFFFFL) return -4;
+    const long z = acc ? 0 : min(grid_limit(256) - T, (V + ZROWS - 1) / ZROWS);
     if (T + z == 0) return 0;
     hipLaunchKernelGGL((small_grad_kernel<TG, W>), dim3((unsigned)(T + z), slabs), dim3(256), 0, st, ids, g, dW,
                        (int)T, V, E, pad, scale, acc);
@@ -600,7 +605,8 @@ int lookup(const Ids& ids, const TW* W, TO* out, long T, long V, int E, float sc
            const float* typ, const Groups& gr, hipStream_t st) {
   const bool vec = E >= 8;
   const int per = vec ? (E + 7) / 8 : E;
-  const int rows = max(1, min(64, 1024 / per));  // about four pieces per thread
+  // about four pieces per thread; more where there are so many tokens that the grid could not hold them
+  const int rows = (int)max(T / grid_limit(256) + 1, (long)max(1, min(64, 1024 / per)));
   const dim3 grid((unsigned)((T + rows - 1) / rows));
   if (vec)
     hipLaunchKernelGGL((lookup_kernel<TW, TO, 8>), grid, dim3(256), 0, st, ids, W, out, T, V, E, scale, rows, pos, typ, gr);
@@ -619,7 +625,7 @@ using namespace pv::temb;
 namespace {
 inline int temb_sizes(long T, long V, long E) {
   if (T < 0 || V <= 0 || E <= 0) return -1;
-  if (T > 0x7FFFFFFFL || V >= 0x7FFFFFFFL || E > (1L << 20)) return -2;
+  if (T > MAX_T || V >= 0x7FFFFFFFL || E > (1L << 20)) return -2;
   return 0;
 }
 }  // namespace

@@ -445,6 +445,9 @@ def trigram_hash(text: torch.Tensor, lens: torch.Tensor, L: int, hash_size: int)
 
 # ---- scaled token lookup, gradient summed over the sorted tokens (csrc/kernels/token_embedding.hip) --------
 
+MAX_TOKENS = (1 << 31) - 1 - 4 * 32  # csrc/kernels/token_embedding.hip::MAX_T
+
+
 def lookup_rows(ids: torch.Tensor, W: torch.Tensor, out: torch.Tensor, scale: float, pos=None, typ0=None,
                 groups=()) -> None:
     """out (T, E) bf16 / fp32 = scale * W[ids] (+ pos[position] + typ0: position of token t of group
@@ -538,7 +541,7 @@ def scaled_embedding(ids: torch.Tensor, W: torch.Tensor, scale: float = 1.0, pad
         return (rows.to(torch.promote_types(W.dtype, torch.float32)) * scale).to(out_dtype)
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"scaled_embedding: out_dtype must be bfloat16 or float32 on the GPU, got {out_dtype}")
-    if W.shape[1] == 0 or V == 0 or ids.numel() >= 1 << 31 or V >= (1 << 31) - 1 or W.shape[1] > 1 << 20:
+    if W.shape[1] == 0 or V == 0 or ids.numel() > MAX_TOKENS or V >= (1 << 31) - 1 or W.shape[1] > 1 << 20:
         raise ValueError(f"scaled_embedding: {ids.numel()} tokens of a {tuple(W.shape)} table are outside the kernels' range")
     ids = ids.contiguous()
     if torch.is_grad_enabled() and W.requires_grad and grad_sink.flat_of(W) is not None:

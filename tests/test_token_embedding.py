@@ -303,3 +303,32 @@ def test_gpu_refusals():
         scaled_embedding(ids, torch.zeros(4, 2, device="cuda"), out_dtype=torch.float16)
     with pytest.raises(ValueError):
         scaled_embedding(ids.cpu(), torch.zeros(4, 2, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_tables_and_token_counts_whose_grid_would_pass_2_to_the_32():
+    """2^30 rows of one column: 2^24 groups of 64 rows to zero.  2^30 tokens of one column."""
+    V = (1 << 30) + 70
+    ids = torch.tensor([3, V - 1, 3, 64, V - 1, 0], device="cuda")
+    W = torch.zeros(V, 1, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    out = scaled_embedding(ids, W, 2.0, padding_idx=0)
+    g = torch.tensor([1.0, 2.0, 4.0, 8.0, 16.0, 32.0], device="cuda").bfloat16().view(6, 1)
+    (dW,) = torch.autograd.grad(out, W, g)
+    assert int(torch.count_nonzero(dW)) == 3
+    assert dW[[3, 64, V - 1], 0].tolist() == [10.0, 16.0, 36.0]
+    del W, dW, out
+    T = (1 << 30) + 70
+    ids = torch.randint(0, 50, (T,), device="cuda", dtype=torch.int32)
+    W = torch.randn(50, 1, device="cuda")
+    out = scaled_embedding(ids, W, 2.0)
+    for part in (slice(0, 1000), slice(T // 2, T // 2 + 1000), slice(T - 1000, T)):
+        assert torch.equal(out[part], (W[ids[part].long()] * 2.0).bfloat16())
+
+
+@pytest.mark.parametrize("T,V,E", [(-1, 5, 4), (5, 0, 4), (5, 5, 0), ((1 << 31) - 128, 5, 4), (5, (1 << 31) - 1, 4), (5, 5, (1 << 20) + 1)])
+def test_sizes_beyond_the_kernels_are_refused(T, V, E):
+    from dnn_page_vectors_amd import _native
+
+    lib = _native.hip(required=True)
+    assert lib.pv_temb_fwd(None, 0, None, 0, None, 0, T, V, E, 1.0, None, None, None, None, 0, None) < 0
+    assert lib.pv_temb_grad(None, 0, None, 0, None, T, V, E, -1, 1.0, 0, None, 0, None) < 0
