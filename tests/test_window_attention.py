@@ -542,3 +542,25 @@ def test_largest_grid_of_short_sequences():
     packed = torch.zeros(1, 3 * d, device="cuda").bfloat16().expand(N + 1, 3 * d)
     with pytest.raises(ValueError):
         packed_window_attention(packed, [None], [(N + 1, 1)], 1, 0, 0)
+
+
+def check_empty(device, dtype):
+    for N, L in ((0, 5), (3, 0)):
+        q, k, v = (torch.zeros(N, L, h, 32, dtype=dtype, device=device).requires_grad_() for h in (4, 2, 2))
+        out = window_attention(q, k, v, 3, 3, 1, torch.ones(N, L, dtype=torch.bool, device=device))
+        assert out.shape == q.shape and out.dtype == dtype
+        for t, g in zip((q, k, v), torch.autograd.grad(out, (q, k, v), torch.zeros_like(out))):
+            assert g.shape == t.shape and g.dtype == dtype
+
+
+def test_empty_results_have_all_gradients_cpu():
+    check_empty("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_empty_results_have_all_gradients():
+    check_empty("cuda", torch.bfloat16)
+    x = torch.zeros(4, 3 * 64, device="cuda").bfloat16().requires_grad_()
+    out = packed_window_attention(x, [None, None], [(2, 2), (0, 7)], 2, 1, 1)
+    (g,) = torch.autograd.grad(out, x, torch.ones_like(out))
+    assert out.shape == (4, 64) and g.shape == x.shape
