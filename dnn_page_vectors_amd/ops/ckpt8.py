@@ -272,7 +272,10 @@ class _Linear8Fn(torch.autograd.Function):
         db = None
         if b is not None and ctx.needs_input_grad[2]:
             tb = grad_sink.write_target(b)
-            db = dops.colsum(dy2, out=tb, accumulate=tb is not None)
+            if dy2.shape[0]:
+                db = dops.colsum(dy2, out=tb, accumulate=tb is not None)
+            else:  # no rows: nothing to add
+                db = torch.zeros(b.shape, dtype=torch.float32, device=dy2.device)
             if tb is not None:
                 grad_sink.done(b)
                 db = None

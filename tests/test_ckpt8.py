@@ -501,3 +501,23 @@ def test_gelu_pack_and_backward_take_any_strides(D):
         ckpt8.ffn(x[:, :32].contiguous(), torch.randn(64, 32).cuda(), torch.randn(64), torch.randn(32, 64).cuda())
     with pytest.raises(TypeError):
         ckpt8.gelu_pack(x.float(), b)
+
+
+def check_no_rows(device, dtype):
+    x = torch.zeros(0, 32, dtype=dtype, device=device).requires_grad_()
+    mk = lambda *s: torch.randn(*s, device=device).requires_grad_()
+    w, b, w2 = mk(16, 32), mk(16), mk(32, 16)
+    for out, ts in ((ckpt8.linear(x, w, b), (x, w, b)), (ckpt8.linear(x, w), (x, w)), (ckpt8.ffn(x, w, b, w2), (x, w, b, w2)),
+                    (ckpt8.bias_gelu(x, torch.zeros(32, device=device)), (x,))):
+        assert out.shape[0] == 0
+        for t, g in zip(ts, torch.autograd.grad(out, ts, torch.zeros_like(out))):
+            assert g.shape == t.shape and not g.any()
+
+
+def test_layers_of_no_rows_cpu():
+    check_no_rows("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_layers_of_no_rows():
+    check_no_rows("cuda", torch.bfloat16)
