@@ -55,6 +55,9 @@ class TwoTowerModel(nn.Module):
     def out_dim(self) -> int:  # pragma: no cover - abstract
         raise NotImplementedError
 
+    def check_device(self, device: torch.device) -> None:
+        """Raises ValueError if this configuration cannot run on ``device`` (the trainer asks before it moves the model)."""
+
     def build_cache(self) -> Dict[str, object]:
         """Derived low-precision copies of the parameters used by the fused kernels."""
         return {}

@@ -30,7 +30,7 @@ import torch.nn.functional as F
 from ..ops import ckpt8, grad_sink
 from ..ops import transformer as tops
 from ..ops.embedding import scaled_embedding
-from ..ops.window_attention import packed_window_attention
+from ..ops.window_attention import HEAD_DIMS, packed_window_attention
 from ..parallel.sparse_rows import note_rows
 from .base import TwoTowerModel
 
@@ -224,6 +224,13 @@ class BertDualEncoder(TwoTowerModel):
     @property
     def out_dim(self) -> int:
         return self.cfg.bert_out_dim or self.cfg.bert_hidden
+
+    def check_device(self, device: torch.device) -> None:
+        cfg = self.cfg
+        d = cfg.bert_hidden // cfg.bert_heads
+        if cfg.bert_window and device.type == "cuda" and cfg.dtype == "bf16" and d not in HEAD_DIMS:
+            raise ValueError(f"bert_window: the GPU's windowed attention takes head dims {HEAD_DIMS}, not "
+                             f"{cfg.bert_hidden} / {cfg.bert_heads} = {d} (bert_hidden / bert_heads)")
 
     def bf16_mirror_params(self):
         return [n for n, _ in self.named_parameters() if n.rsplit(".", 1)[-1] in ("wqkv", "wo", "w1", "w2")]

@@ -101,6 +101,8 @@ class Trainer:
         self.cfg = cfg
         self.info = pdist.info()
         self.device = device or self.info.device
+        if hasattr(model, "check_device"):
+            model.check_device(self.device)
         self.model = model.to(self.device)
         self.flat = FlatParams(self.model.named_parameters())
         broadcast_params(self.flat)

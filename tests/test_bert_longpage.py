@@ -267,3 +267,15 @@ def test_position_and_type_gradients(groups):
     assert not dtyp[1].any()
     again = tops._position_grads(g.cuda(), groups, pos, typ, True, True)
     assert torch.equal(dpos, again[0]) and torch.equal(dtyp, again[1])
+
+
+def test_head_dims_that_the_gpu_refuses_are_found_before_the_first_step():
+    """96 columns in 4 heads of 24: the CPU form takes them, a trainer on the GPU says so when it is made."""
+    bad = config(bert_hidden=96, bert_heads=4)
+    m = build_model(bad, 400)
+    with pytest.raises(ValueError, match="head dims"):
+        Trainer(bad, m, torch.device("cuda:0"))
+    out = Trainer(bad, m, torch.device("cpu")).train_step(*SyntheticPairs(spec_from_config(bad, 400, num_pages=64)).batch(8))
+    assert float(out["loss"]) == float(out["loss"])
+    for fine in (bad.replace(bert_window=0), bad.replace(dtype="fp32"), config()):
+        build_model(fine, 400).check_device(torch.device("cuda:0"))
