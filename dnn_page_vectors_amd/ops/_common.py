@@ -110,6 +110,15 @@ def on_device(t: torch.Tensor):
     return contextlib.nullcontext()
 
 
+def refuse_held_capture(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Inside a capture: RuntimeError if an eager graph made on another stream still holds one of these leaves (autograd
+    would wait for that stream in the captured backward, which ends the process; csrc/binding/autograd.cpp)."""
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        for t in tensors:
+            if t is not None:
+                _native.binding().check_capture(t, what)
+
+
 def P(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

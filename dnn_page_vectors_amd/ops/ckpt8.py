@@ -25,7 +25,7 @@ from .. import _native
 from . import dense as dops
 from . import grad_sink
 from . import transformer as tops
-from ._common import P, check, lib, on_device, stream, use_hip
+from ._common import P, check, lib, on_device, refuse_held_capture, stream, use_hip
 
 BLOCK = 32
 FP8_MAX = 448.0
@@ -242,6 +242,8 @@ def bias_gelu(x: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
         return _gelu_alone(x, b)
     if use_hip(x) and grad_sink.flat_of(b) is None:
         return _native.binding().bias_gelu8(x, b)
+    if use_hip(x):
+        refuse_held_capture("ckpt8.bias_gelu", x, b)
     return _BiasGelu8Fn.apply(x, b)
 
 
@@ -321,6 +323,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None,
     if not (torch.is_grad_enabled() and w.requires_grad):
         return tops.linear(x, w, b, res=res)
     if use_hip(x):
+        refuse_held_capture("ckpt8.linear", x, w, b)
         return _Linear8Fn.apply(x, w, b, tops.weight_bf16(w), res)
     y = _RoundSaved.apply(x, w)
     return y if b is None else y + b.to(y.dtype)
@@ -368,5 +371,6 @@ def ffn(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w1, b1, w2))):
         return tops.linear(_gelu_alone(tops.linear(x, w1, res=res), b1), w2)
     if use_hip(x):
+        refuse_held_capture("ckpt8.ffn", x, w1, b1, w2)
         return _FFN8Fn.apply(x, w1, b1, w2, tops.weight_bf16(w1), tops.weight_bf16(w2), res)
     return _RoundSaved.apply(bias_gelu(_RoundSaved.apply(x, w1), b1), w2)

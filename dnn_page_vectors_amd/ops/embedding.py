@@ -28,7 +28,7 @@ from .. import _native
 from . import dense as dops
 from . import grad_sink
 from . import reference as ref
-from ._common import P, check, lib, on_device, stream, use_hip
+from ._common import P, check, lib, on_device, refuse_held_capture, stream, use_hip
 from ..parallel.sparse_rows import note_rows
 from .conv_pool import sort_pairs_iota
 
@@ -545,6 +545,7 @@ def scaled_embedding(ids: torch.Tensor, W: torch.Tensor, scale: float = 1.0, pad
         raise ValueError(f"scaled_embedding: {ids.numel()} tokens of a {tuple(W.shape)} table are outside the kernels' range")
     ids = ids.contiguous()
     if torch.is_grad_enabled() and W.requires_grad and grad_sink.flat_of(W) is not None:
+        refuse_held_capture("scaled_embedding", W)
         return _ScaledEmbeddingFn.apply(W, ids, float(scale), padding_idx, out_dtype)
     return _native.binding().scaled_embedding(W, ids, float(scale), -1 if padding_idx is None else int(padding_idx),
                                               out_dtype == torch.bfloat16)

@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from . import dense as dops
 from . import grad_sink
 from . import reference as ref
-from ._common import P, check, lib, stream, use_hip
+from ._common import P, check, lib, refuse_held_capture, stream, use_hip
 
 
 def _seed_ptr():
@@ -506,6 +506,7 @@ def bert_embed(word: torch.Tensor, pos: torch.Tensor, typ: torch.Tensor, ids_lis
     if scale:
         if not (use_hip(word) and word.dtype == torch.float32 and len(ids_list) <= 4):
             return None
+        refuse_held_capture("bert_embed", word, pos, typ)
         from ..parallel.sparse_rows import note_rows
 
         flat = torch.cat([i.reshape(-1) for i in ids_list]) if len(ids_list) > 1 else ids_list[0].reshape(-1).contiguous()

@@ -19,7 +19,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .. import _native
-from ._common import P, check, lib, on_device, stream, use_hip
+from ._common import P, check, lib, on_device, refuse_held_capture, stream, use_hip
 
 HEAD_DIMS = (32, 64, 128)
 MAX_LEN = 1 << 29
@@ -234,7 +234,7 @@ def packed_window_attention(qkv: torch.Tensor, masks: Sequence[Optional[torch.Te
             _check_range(N, L, heads)
         train = torch.is_grad_enabled() and qkv.requires_grad
         if train:
-            _native.binding().check_capture(qkv, "packed_window_attention")
+            refuse_held_capture("packed_window_attention", qkv)
         return _PackedWindowAttnFn.apply(qkv, masks, shapes, heads, (left, right, sinks), _scale(None, d), train)
     outs, off = [], 0
     for (N, L), m in zip(shapes, masks):

@@ -128,3 +128,51 @@ def test_forward_mode_cpu(name):
     with torch.autograd.forward_ad.dual_level():
         out = torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))))
         assert out.tangent is not None and out.tangent.abs().max() > 0
+
+
+def capture_calls():
+    """Differentiable calls of the Python nodes: (function, its leaves, which of them a backward can reach)."""
+    from dnn_page_vectors_amd.ops import ckpt8
+    from dnn_page_vectors_amd.ops import transformer as tops
+    from dnn_page_vectors_amd.ops.embedding import scaled_embedding
+    from dnn_page_vectors_amd.ops.optim import FlatParams
+
+    mk = lambda *s: torch.nn.Parameter(torch.randn(*s, device="cuda") * 0.1)
+    x = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_()
+    w1, b1, w2 = mk(96, 64), mk(96), mk(64, 96)
+    word, pos, typ = mk(50, 64), mk(20, 64), mk(2, 64)
+    flat_word, flat_bias = mk(50, 64), mk(64)
+    FlatParams([("w", flat_word), ("b", flat_bias)])
+    ids = torch.randint(0, 50, (4, 10), device="cuda")
+    return {
+        "linear": (lambda: ckpt8.linear(x, w1, b1), (x, w1, b1)),
+        "ffn": (lambda: ckpt8.ffn(x, w1, b1, w2), (x, w1, b1, w2)),
+        "embed": (lambda: tops.bert_embed(word, pos, typ, [ids], 2.0), (word, pos, typ)),
+        "flat table": (lambda: scaled_embedding(ids, flat_word, 2.0), (flat_word,)),
+        "flat bias": (lambda: ckpt8.bias_gelu(x, flat_bias), (x, flat_bias)),
+    }
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["linear", "ffn", "embed", "flat table", "flat bias"])
+def test_python_nodes_refuse_a_capture_over_held_leaves(name):
+    """As the C++ nodes do: nothing is captured, and once the eager graph is gone the capture works."""
+    f, leaves = capture_calls()[name]
+    held = f()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            f()
+    del held
+    dy = torch.randn_like(f().detach())
+    want = torch.autograd.grad(f(), leaves, dy, allow_unused=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(f(), leaves, dy, allow_unused=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            assert (a is None) == (c is None)   # a flat parameter's gradient is written in place
+            # a bias of the linear layer is summed by atomics: any order of 40 terms
+            assert a is None or torch.allclose(a, c, rtol=1e-4, atol=40 * 2.0 ** -23 * float(dy.float().abs().sum(0).max()))
