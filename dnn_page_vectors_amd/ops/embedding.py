@@ -448,16 +448,39 @@ def trigram_hash(text: torch.Tensor, lens: torch.Tensor, L: int, hash_size: int)
 MAX_TOKENS = (1 << 31) - 1 - 4 * 32  # csrc/kernels/token_embedding.hip::MAX_T
 
 
+def _check_rows(name: str, ids: torch.Tensor, table: torch.Tensor, rows: torch.Tensor) -> None:
+    """What the kernels behind raw pointers take: contiguous int32 / int64 ids, one row of bf16 / fp32 each."""
+    if ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous():
+        raise TypeError(f"{name}: ids must be contiguous int32 or int64, got {ids.dtype}")
+    if table.dim() != 2 or rows.shape != (ids.numel(), table.shape[1]):
+        raise ValueError(f"{name}: {ids.numel()} ids, rows {tuple(rows.shape)} and a table {tuple(table.shape)} do not fit")
+    if rows.dtype not in (torch.bfloat16, torch.float32) or not rows.is_contiguous():
+        raise TypeError(f"{name}: rows must be contiguous bfloat16 or float32, got {rows.dtype}")
+    if not ids.device == table.device == rows.device:
+        raise ValueError(f"{name}: ids are on {ids.device}, the table on {table.device}, the rows on {rows.device}")
+
+
 def lookup_rows(ids: torch.Tensor, W: torch.Tensor, out: torch.Tensor, scale: float, pos=None, typ0=None,
                 groups=()) -> None:
     """out (T, E) bf16 / fp32 = scale * W[ids] (+ pos[position] + typ0: position of token t of group
     (N_i, L_i) of the packed ids = its place in its sequence).  One launch."""
     import ctypes
 
+    _check_rows("lookup_rows", ids, W, out)
+    if W.dtype not in (torch.float32, torch.bfloat16) or not W.is_contiguous():
+        raise TypeError(f"lookup_rows: the table must be contiguous float32 or bfloat16, got {W.dtype}")
     offs, off = [], 0
     for N, L in groups:
         offs.append(off)
         off += N * L
+    if pos is not None:
+        most = max((L for _, L in groups), default=0)
+        if off != ids.numel() or not 1 <= len(offs) <= 4:
+            raise ValueError(f"lookup_rows: groups {list(groups)} do not cover {ids.numel()} tokens (1 to 4 of them)")
+        for t, shape in ((pos, (max(most, pos.shape[0]), W.shape[1])), (typ0, (W.shape[1],))):
+            if t is None or t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != W.device:
+                raise ValueError(f"lookup_rows: position rows (at least {most}) and the type row must be contiguous float32 "
+                                 f"of {W.shape[1]} columns on {W.device}")
     oa = (ctypes.c_int * len(offs))(*offs) if offs else None
     la = (ctypes.c_int * len(offs))(*[L for _, L in groups]) if offs else None
     with on_device(W):
@@ -473,6 +496,9 @@ def sorted_row_grad(ids: torch.Tensor, g: torch.Tensor, dst: torch.Tensor, scale
     and ids outside the table add nothing."""
     T, E = g.shape
     V = dst.shape[0]
+    _check_rows("sorted_row_grad", ids, dst, g)
+    if dst.dtype != torch.float32 or not dst.is_contiguous():
+        raise TypeError(f"sorted_row_grad: the gradient must be contiguous float32, got {dst.dtype}")
     with on_device(dst):
         n = int(lib().pv_temb_grad_ws(T, V, E))
         ws = torch.empty(n, dtype=torch.uint8, device=dst.device) if n else None

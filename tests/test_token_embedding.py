@@ -332,3 +332,56 @@ def test_sizes_beyond_the_kernels_are_refused(T, V, E):
     lib = _native.hip(required=True)
     assert lib.pv_temb_fwd(None, 0, None, 0, None, 0, T, V, E, 1.0, None, None, None, None, 0, None) < 0
     assert lib.pv_temb_grad(None, 0, None, 0, None, T, V, E, -1, 1.0, 0, None, 0, None) < 0
+
+
+F = lambda *s: torch.zeros(*s)
+I = lambda *s: torch.zeros(*s, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("call", [
+    lambda e: e.lookup_rows(F(4), F(9, 8), F(4, 8), 1.0),
+    lambda e: e.lookup_rows(I(8)[::2], F(9, 8), F(4, 8), 1.0),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(5, 8), 1.0),
+    lambda e: e.lookup_rows(I(4), F(9, 8).t(), F(4, 9), 1.0),
+    lambda e: e.lookup_rows(I(4), F(9, 8).double(), F(4, 8), 1.0),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8).half(), 1.0),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8, ).to("meta"), 1.0),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8), 1.0, F(6, 8), F(8), [(1, 3)]),
+    lambda e: e.lookup_rows(I(5), F(9, 8), F(5, 8), 1.0, F(6, 8), F(8), [(1, 1)] * 5),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8), 1.0, F(1, 8), F(8), [(2, 2)]),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8), 1.0, F(6, 8).bfloat16(), F(8), [(2, 2)]),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8), 1.0, F(6, 8), None, [(2, 2)]),
+    lambda e: e.lookup_rows(I(4), F(9, 8), F(4, 8), 1.0, F(6, 8), F(7), [(2, 2)]),
+    lambda e: e.sorted_row_grad(I(4), F(5, 8), F(9, 8), 1.0, None, False),
+    lambda e: e.sorted_row_grad(I(4), F(4, 7), F(9, 8), 1.0, None, False),
+    lambda e: e.sorted_row_grad(I(4), F(4, 8).double(), F(9, 8), 1.0, None, False),
+    lambda e: e.sorted_row_grad(I(4), F(4, 8), F(9, 8).bfloat16(), 1.0, None, False),
+    lambda e: e.sorted_row_grad(I(4), F(4, 16)[:, ::2], F(9, 8), 1.0, None, False),
+])
+def test_refused_operands_of_the_row_functions(call):
+    from dnn_page_vectors_amd.ops import embedding
+
+    with pytest.raises((TypeError, ValueError)):
+        call(embedding)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E", [5, 64, 770])
+@pytest.mark.parametrize("groups", [[(1, 1)], [(3, 7), (2, 40)], [(1, 300), (0, 5), (4, 0), (9, 31)]])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_lookup_with_position_and_type_rows(E, groups, out):
+    """round(scale W[id] + pos[l] + typ): three fp32 roundings, each of at most the magnitudes' sum, and the last."""
+    from dnn_page_vectors_amd.ops.embedding import lookup_rows
+
+    gen = torch.Generator().manual_seed(E)
+    V, T = 60, sum(N * L for N, L in groups)
+    W, pos, typ = torch.randn(V, E, generator=gen), torch.randn(300, E, generator=gen), torch.randn(E, generator=gen)
+    ids = torch.randint(0, V, (T,), generator=gen)
+    where = torch.cat([torch.arange(L).repeat(N) for N, L in groups])
+    got = torch.empty(T, E, dtype=out, device="cuda")
+    lookup_rows(ids.cuda(), W.cuda(), got, 1.7, pos.cuda(), typ.cuda(), groups)
+    scale = float(torch.tensor(1.7))
+    parts = (scale * W.double()[ids], pos.double()[where], typ.double().expand(T, E))
+    want, mag = sum(parts), sum(p.abs() for p in parts)
+    last = 2.0 ** -8 if out == torch.bfloat16 else 0.0
+    assert ((got.double().cpu() - want).abs() <= (3 * 2.0 ** -24 * mag) * (1 + last) + last * want.abs()).all()
