@@ -37,8 +37,8 @@ def _window(left: Optional[int], right: Optional[int], sinks: int, L: int) -> Tu
 
 def _scale(scale: Optional[float], d: int) -> float:
     s = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not (s > 0.0 and math.isfinite(s)):
-        raise ValueError(f"window_attention: scale must be positive and finite, got {scale!r}")
+    if not 2.0 ** -126 <= s <= 2.0 ** 120:  # times log2(e) it has to stay a finite, normal fp32 number
+        raise ValueError(f"window_attention: scale must be positive and finite (2^-126 to 2^120), got {scale!r}")
     return s
 
 

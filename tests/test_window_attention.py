@@ -564,3 +564,20 @@ def test_empty_results_have_all_gradients():
     out = packed_window_attention(x, [None, None], [(2, 2), (0, 7)], 2, 1, 1)
     (g,) = torch.autograd.grad(out, x, torch.ones_like(out))
     assert out.shape == (4, 64) and g.shape == x.shape
+
+
+@pytest.mark.parametrize("scale", [1e-46, 2.0 ** -127, 2.0 ** 121, 1e39, 1e300])
+def test_scales_that_fp32_does_not_hold_are_refused(scale):
+    q = torch.zeros(1, 2, 1, 8)
+    with pytest.raises(ValueError, match="scale"):
+        window_attention(q, q, q, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -20, 2.0 ** 40])
+def test_extreme_scales(scale):
+    """Scores of at most 2^4 whatever the scale: the factor goes into the queries."""
+    q, k, v, do = inputs(2, 70, 2, 2, 64, 9)
+    big = (q.float() / 16 / scale).clamp(-2.0 ** 100, 2.0 ** 100).bfloat16()
+    want, tol = oracle(big, k, v, do, 9, 9, 1, None, scale)
+    close(window_attention(big, k, v, 9, 9, 1, None, scale), want[0], tol[0], "out")
