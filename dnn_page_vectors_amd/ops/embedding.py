@@ -563,8 +563,15 @@ def scaled_embedding(ids: torch.Tensor, W: torch.Tensor, scale: float = 1.0, pad
         out_dtype = torch.bfloat16 if use_hip(W) else W.dtype
     note_rows(W, ids)  # row-sparse table gradients (parallel/sparse_rows.py) record the rows
     if not use_hip(W):
-        rows = torch.nn.functional.embedding(ids.long(), W, padding_idx=padding_idx)
-        return (rows.to(torch.promote_types(W.dtype, torch.float32)) * scale).to(out_dtype)
+        ids = ids.long()
+        if W.is_cuda:  # torch's lookup would stop the device at an id outside the table
+            ok = (ids >= 0) & (ids < V)
+            ids = ids.masked_fill(~ok, 0)
+        rows = torch.nn.functional.embedding(ids, W, padding_idx=padding_idx)
+        rows = rows.to(torch.promote_types(W.dtype, torch.float32)) * scale
+        if W.is_cuda:
+            rows = rows.masked_fill(~ok.unsqueeze(-1), float("nan"))
+        return rows.to(out_dtype)
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"scaled_embedding: out_dtype must be bfloat16 or float32 on the GPU, got {out_dtype}")
     if W.shape[1] == 0 or V == 0 or ids.numel() > MAX_TOKENS or V >= (1 << 31) - 1 or W.shape[1] > 1 << 20:

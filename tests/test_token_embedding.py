@@ -385,3 +385,23 @@ def test_lookup_with_position_and_type_rows(E, groups, out):
     want, mag = sum(parts), sum(p.abs() for p in parts)
     last = 2.0 ** -8 if out == torch.bfloat16 else 0.0
     assert ((got.double().cpu() - want).abs() <= (3 * 2.0 ** -24 * mag) * (1 + last) + last * want.abs()).all()
+
+
+@pytest.mark.gpu
+def test_ids_outside_the_table_without_the_kernels():
+    """The plain form on the GPU (dtype="fp32", backend "torch"): a row of NaN, no gradient, no device assertion."""
+    from dnn_page_vectors_amd.ops import _common
+
+    W = torch.randn(20, 6, device="cuda").requires_grad_()
+    ids = torch.tensor([3, -1, 20, 3, 1 << 40, 0], device="cuda")
+    before = _common.get_backend()
+    _common.set_backend("torch")
+    try:
+        out = scaled_embedding(ids, W, 2.0, padding_idx=0)
+        (dW,) = torch.autograd.grad(out, W, torch.ones_like(out))
+    finally:
+        _common.set_backend(before)
+    assert out[[1, 2, 4]].isnan().all() and torch.equal(out[[0, 3, 5]], 2 * W[[3, 3, 0]])
+    want = torch.zeros_like(W)
+    want[3] = 4
+    assert torch.equal(dW, want)
