@@ -816,6 +816,10 @@ __host__ inline int check_sizes(long N, long L, long H, long G, int d, float sca
   return grid_holds((L + RB - 1) / RB * H * N, L) ? 0 : -4;
 }
 
+// A row's offset within a tile of 64 is 32 bits of bytes: strides of the rows that tiles are read from (the l-th of the
+// three of operand i)
+__host__ inline bool tiles_hold(const long* st, int i) { return st[3 * i + 1] < (1L << 25); }
+
 // The far part of the sinks is split off where they all lie in the first workgroup of keys and it is long
 // enough to matter (8 tiles; forward and backward of 64 pages x 12 heads x 64, window 128 + 128, one sink, split / not:
 // 5 tiles behind the window 356 / 352 us, 9 tiles 484 / 484, 15 tiles 682 / 715; 2 pages of 4096: 117 / 200).  More
@@ -875,6 +879,7 @@ PV_API int pv_wattn_fwd(const void* q, const void* k, const void* v, void* o, co
                         int left, int right, int sinks, float scale, void* stream) {
   if (const int rc = check_sizes(N, L, H, G, d, scale)) return rc;
   if (!lse != !rest) return -5;
+  if (!tiles_hold(st, 1) || !tiles_hold(st, 2)) return -6;
   const Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, rest, L, H, G, left, right, sinks, scale);
   const dim3 grid((unsigned)((long)a.tiles * H * N));
   hipStream_t s = (hipStream_t)stream;
@@ -903,6 +908,8 @@ PV_API int pv_wattn_bwd(const void* q, const void* k, const void* v, const void*
                         const void* rest, float* dd, float* ws, long ws_floats, int N, int L, int H, int G, int d, int left, int right, int sinks,
                         float scale, void* stream) {
   if (const int rc = check_sizes(N, L, H, G, d, scale)) return rc;
+  for (const int i : {0, 1, 2, 4})  // q, k, v, go
+    if (!tiles_hold(st, i)) return -6;
   Args a = common(q, k, v, o, st, mask, mask_n, mask_bytes, lse, const_cast<void*>(rest), L, H, G, left, right, sinks,
                   scale);
   a.go = view(go, st, 4);

@@ -56,9 +56,11 @@ def _key_mask(mask: Optional[torch.Tensor], N: int, L: int, device) -> Optional[
     return mask if L == 1 or mask.stride(1) == 1 else mask.contiguous()
 
 
-def _check_range(N: int, L: int, H: int) -> None:
+def _check_range(N: int, L: int, H: int, d: int = 0) -> None:
     """A workgroup per 128 queries and head, of 128 threads for up to 64 tokens and 256 above, in a grid of fewer than
-    2^32 threads."""
+    2^32 threads; offsets within a tile of 64 rows in 32 bits."""
+    if H * d >= 1 << 24:
+        raise ValueError(f"window_attention: {H} heads of {d} columns are outside the kernels' range (2^24 columns)")
     if L > MAX_LEN or N * H * -(-L // 128) * (128 if L <= 64 else 256) >= 1 << 32:
         raise ValueError(f"window_attention: {N} sequences of {L} tokens and {H} heads are outside the kernels' range "
                          f"(length {MAX_LEN}, 2^25 heads of up to 64 tokens, 2^24 blocks of 128 queries of longer ones)")
@@ -161,7 +163,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
         raise TypeError(f"window_attention: the GPU kernels take bfloat16, got {q.dtype}")
     if d not in HEAD_DIMS:
         raise ValueError(f"window_attention: head dim must be one of {HEAD_DIMS} on the GPU, got {d}")
-    _check_range(N, L, H)
+    _check_range(N, L, H, d)
     if q.numel() == 0:
         return q * 1.0 + (k.sum() + v.sum())  # nothing to add, but a result of all three
     return _native.binding().window_attention(q, k, v, mask, *win, scale)

@@ -581,3 +581,29 @@ def test_extreme_scales(scale):
     big = (q.float() / 16 / scale).clamp(-2.0 ** 100, 2.0 ** 100).bfloat16()
     want, tol = oracle(big, k, v, do, 9, 9, 1, None, scale)
     close(window_attention(big, k, v, 9, 9, 1, None, scale), want[0], tol[0], "out")
+
+
+def test_rows_too_far_apart_for_32_bit_tile_offsets_are_refused():
+    """63 rows of 2^25 columns are 2^32 bytes: the last rows of a tile would be read from its beginning."""
+    from dnn_page_vectors_amd import _native
+    from dnn_page_vectors_amd.ops.window_attention import _check_range
+
+    with pytest.raises(ValueError):
+        _check_range(1, 65, 1 << 18, 64)
+    _check_range(1, 65, (1 << 18) - 1, 64)
+    lib = _native.hip(required=True)
+    for i in (1, 2):
+        st = (ctypes.c_long * 12)(*[64] * 12)
+        st[3 * i + 1] = 1 << 25
+        assert lib.pv_wattn_fwd(None, None, None, None, st, None, 0, 1, None, None, 1, 65, 1, 1, 64, 1, 1, 0, 0.5, None) == -6
+    for i in (0, 1, 2, 4):
+        st = (ctypes.c_long * 24)(*[64] * 24)
+        st[3 * i + 1] = 1 << 25
+        assert lib.pv_wattn_bwd(*[None] * 8, st, None, 0, 1, None, None, None, None, 0, 1, 65, 1, 1, 64, 1, 1, 0, 0.5, None) == -6
+
+
+@pytest.mark.gpu
+def test_too_many_columns_are_refused():
+    q = torch.zeros(1, 1, 1, 64, device="cuda").bfloat16().expand(1, 65, 1 << 18, 64)
+    with pytest.raises(ValueError):
+        window_attention(q, q, q, 3, 3)
