@@ -1,4 +1,5 @@
-// Autograd nodes of the latency-bound operators in C++ (Python module pagevec_torch).
+// Autograd nodes in C++ (Python module pagevec_torch) of the operators called by themselves; the transformer tower's own
+// layers are Python nodes over the same kernels (ops/*.py).
 //
 // A Python autograd.Function around two small kernels costs about 100 us of host time per forward and
 // backward on this host (the backward runs on the engine's device thread, which has to take the

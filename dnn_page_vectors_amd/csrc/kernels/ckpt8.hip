@@ -184,7 +184,7 @@ __device__ __forceinline__ Place place(const Shape& s) {
 }
 // Bound by memory: 256000 x 768 bf16 in 134 us (4.4 TB/s), with bias and GELU 73728 x 2048 in 148 (5.1 TB/s); a
 // column per lane instead of 8 took 348 against 114 us at 73728 x 2047.  Slabs of columns that leave fewer threads
-// idle than whole rows do (96 of 256 are, at 768) were no faster: 202 -> 218 us with GELU.
+// idle than whole rows do (64 of 256 are, at 768) were no faster: 202 -> 218 us with GELU.
 // MODE 0: pack x;  1: u = x + b, y = gelu(u), pack u.  U rows in flight per thread.
 template <typename T, int MODE, int U, bool ODD>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, const float* __restrict__ b,

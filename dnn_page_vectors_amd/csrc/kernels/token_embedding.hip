@@ -22,7 +22,7 @@ namespace temb {
 // Up to here one launch, which compares every token with all others: at 4096 tokens 18 / 23 / 48 / 42 us where sorting
 // takes 31 / 31 / 43 / 50 (tables of 5000 x 64, 1024 x 300, 30522 x 768, 60000 x 512, Zipf ids), at 8192 30 / 45 / 94 / 75
 // against 33 / 32 / 48 / 53; the sort's five further launches cost another 15 us of host time.  The worst ids, all
-// the same: 173 against 29 us at 4096 tokens.
+// the same: 173 against 29 us at 4096 tokens (a padded batch whose padding is not excluded comes near).
 constexpr int SMALL_T = 4096;
 constexpr int CHUNK = 32;  // sorted tokens per wave
 constexpr long MAX_T = 0x7FFFFFFFL - 4 * CHUNK;  // token numbers in 31 bits, and a grid of fewer than 2^32 threads for them
