@@ -95,6 +95,13 @@ class PhaseTimer:
         return out
 
 
+def _capture_error_mode() -> str:
+    """With a process group, its watchdog thread still asks for the events of the last steps' collectives (it looks every
+    100 ms).  In the "global" mode a capture forbids that to every thread, and the watchdog then ends the
+    process; "thread_local" forbids it to the capturing thread alone."""
+    return "thread_local" if torch.distributed.is_initialized() else "global"
+
+
 class Trainer:
     def __init__(self, cfg, model: TwoTowerModel, device: Optional[torch.device] = None,
                  metrics: Optional[MetricsLogger] = None, graph: bool = False, graph_fence: bool = False):
@@ -377,7 +384,7 @@ class Trainer:
         g = torch.cuda.CUDAGraph()
         cops.set_seed_tensor(self._seed_dev)  # conv kernels add the per-replay device seed
         try:
-            with torch.cuda.graph(g):
+            with torch.cuda.graph(g, capture_error_mode=_capture_error_mode()):
                 self._gout = self._eager_step(self._gq, self._gd, seed_override=0, timing=False)
         finally:
             cops.set_seed_tensor(None)

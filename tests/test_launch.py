@@ -103,3 +103,18 @@ def test_comm_micro_gloo_and_channel_sweep():
     assert len(recs) == 2 * 3  # per channel setting: 1 all-reduce + 2 all-gathers
     assert {x["env"].get("NCCL_MIN_NCHANNELS") for x in recs} == {"2", "4"}
     assert all(x["world"] == 2 and x["ms"] > 0 for x in recs)
+
+
+def test_captures_leave_the_watchdog_alone():
+    """Where a process group lives, a capture forbids unsafe calls to its own thread only."""
+    import torch.distributed as dist
+
+    from dnn_page_vectors_amd.train.trainer import _capture_error_mode
+
+    assert not dist.is_initialized() and _capture_error_mode() == "global"
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        assert _capture_error_mode() == "thread_local"
+    finally:
+        dist.destroy_process_group()
+    assert _capture_error_mode() == "global"
