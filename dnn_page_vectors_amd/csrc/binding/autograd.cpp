@@ -16,6 +16,7 @@
 
 #include <optional>
 #include <string>
+#include <vector>
 
 namespace {
 
@@ -101,6 +102,21 @@ void check_capture(std::initializer_list<const Tensor*> ts, const char* what) {
     TORCH_CHECK(s && *s == c10::hip::getCurrentHIPStream(t->get_device()).unwrap(), what,
                 ": a graph made on another stream still holds an argument of this capture (delete its outputs first)");
   }
+}
+
+// Memset nodes of a captured graph (a hipGraph_t).  Replays after the first have run such nodes wrongly.
+int64_t graph_memsets(size_t graph) {
+  size_t n = 0;
+  TORCH_CHECK(hipGraphGetNodes(reinterpret_cast<hipGraph_t>(graph), nullptr, &n) == hipSuccess, "hipGraphGetNodes failed");
+  std::vector<hipGraphNode_t> nodes(n);
+  if (n) TORCH_CHECK(hipGraphGetNodes(reinterpret_cast<hipGraph_t>(graph), nodes.data(), &n) == hipSuccess, "hipGraphGetNodes failed");
+  int64_t sets = 0;
+  for (const hipGraphNode_t node : nodes) {
+    hipGraphNodeType type;
+    TORCH_CHECK(hipGraphNodeGetType(node, &type) == hipSuccess, "hipGraphNodeGetType failed");
+    sets += type == hipGraphNodeTypeMemset;
+  }
+  return sets;
 }
 
 // ---- windowed attention ------------------------------------------------------------------------------------------
@@ -321,5 +337,6 @@ PYBIND11_MODULE(pagevec_torch, m) {
     check_capture({&x, &b}, "ckpt8.bias_gelu");
     return Tensor(BiasGelu8::apply(x, b));
   }, call_guard<gil_scoped_release>());
+  m.def("graph_memsets", &graph_memsets);
   m.def("check_capture", [](const Tensor& t, const char* what) { check_capture({&t}, what); });
 }

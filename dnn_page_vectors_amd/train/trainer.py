@@ -27,6 +27,7 @@ from typing import Callable, Dict, Iterable, Iterator, List, Optional, Tuple
 
 import torch
 
+from .. import _native
 from ..models.base import TwoTowerModel, bump_generation
 from ..ops import dense as dops
 from ..ops import determinism
@@ -381,7 +382,7 @@ class Trainer:
         self._seed_dev = torch.zeros(1, dtype=torch.int32, device=self.device)
         torch.cuda.synchronize()
         step0, count0 = self.step, self.opt.step_count
-        g = torch.cuda.CUDAGraph()
+        g = torch.cuda.CUDAGraph(keep_graph=True)
         cops.set_seed_tensor(self._seed_dev)  # conv kernels add the per-replay device seed
         try:
             with torch.cuda.graph(g, capture_error_mode=_capture_error_mode()):
@@ -390,6 +391,15 @@ class Trainer:
             cops.set_seed_tensor(None)
         # the capture only recorded the step: undo its host-side bookkeeping
         self.step, self.opt.step_count = step0, count0
+        if self.sparse is None or getattr(self.cfg, "dtype", "bf16") == "fp32":
+            # torch's sums over many rows clear counters by a memset, and replays after the first gave the fp32
+            # transformer bias gradients that were wrong by orders of magnitude.  The HIP kernels' steps hold none
+            # but the row-sparse exchange's, whose replays are tested against eager steps.
+            memsets = _native.binding().graph_memsets(g.raw_cuda_graph())
+            if memsets:
+                self._gout = None
+                raise RuntimeError(f"the step holds {memsets} memsets, which graph replays do not repeat reliably")
+        g.instantiate()
         self._graph, self._graph_key = g, key
 
     def _event(self) -> torch.cuda.Event:

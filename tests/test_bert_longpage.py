@@ -279,3 +279,44 @@ def test_head_dims_that_the_gpu_refuses_are_found_before_the_first_step():
     assert float(out["loss"]) == float(out["loss"])
     for fine in (bad.replace(bert_window=0), bad.replace(dtype="fp32"), config()):
         build_model(fine, 400).check_device(torch.device("cuda:0"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,status", [("bf16", "captured"), ("fp32", "eager")])
+def test_steps_with_memsets_are_not_replayed(dtype, status):
+    """dtype="fp32" runs torch's own sums, whose memsets replays repeat wrongly (bias gradients off by orders of
+    magnitude): the trainer keeps such a step eager and says so.  The gradients are then those of a trainer without graphs."""
+    kw = dict(dtype=dtype, loss_mode="in_batch", bert_max_len=2000, document_length=300, bert_hidden=256, bert_heads=4)
+    dev = torch.device("cuda:0")
+    grads = []
+    for graph in (True, False):
+        cfg = config(lr=0.0, **kw)                   # the weights stay: every step of a batch has the same gradient
+        tr = Trainer(cfg, build_model(cfg, 400), dev, graph=graph)
+        for seed in range(6):
+            q, d = pair_batch(cfg, dev, seed=seed)
+            tr.train_step(q, d)
+        torch.cuda.synchronize()
+        assert tr.graph_status.startswith(status if graph else "off")
+        assert (tr._graph is not None) == (graph and status == "captured")
+        grads.append(tr.flat.grad.clone())
+        tr.close()
+    a, b = grads
+    assert torch.isfinite(a).all() and b.abs().max() > 0
+    # sums of the same terms in another order (atomics)
+    assert float((a - b).norm()) <= 1e-3 * float(b.norm())
+
+
+@pytest.mark.gpu
+def test_memset_nodes_are_counted():
+    from dnn_page_vectors_amd import _native
+
+    x = torch.randn(4000, 256, device="cuda")
+    for f, sets in ((lambda: x * 2, 0), (lambda: x.sum(0), 1)):
+        f()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            y = f()
+        kinds = node_kinds(graph)
+        assert _native.binding().graph_memsets(graph.raw_cuda_graph()) == kinds.get(2, 0) == sets
+        del y
